@@ -90,7 +90,9 @@ enum tcg_opcode
 	TCG_SUB, TCG_MUL, TCG_DIV, TCG_MIN, TCG_MAX, TCG_EQ, TCG_NEQ, TCG_LT,
 	TCG_GT, TCG_MATMUL, TCG_CONTRACT, TCG_CONV, TCG_SELECT, TCG_CONCAT,
 	TCG_ASSIGN, TCG_ASSIGN_ADD, TCG_ASSIGN_SUB, TCG_ASSIGN_MUL, TCG_ASSIGN_DIV,
-	TCG_CAST, TCG_N_OPCODES
+	TCG_CAST,
+	/* nodes of this backend's graphs that cfg/ops.yml does not have */
+	TCG_LAYER_NORM, TCG_LAYER_NORM_DX, TCG_LAYER_NORM_DWEIGHT, TCG_N_OPCODES
 };
 
 /* ---- context, memory, transfers -------------------------------------- */
@@ -647,6 +649,37 @@ int tcg_conv_views (tcg_ctx* ctx, int dtype, const uint64_t imgshape[8],
  * No counterpart in the reference; for tests and for callers who want to know
  * which route their shapes take. */
 int tcg_conv_route_counts (const tcg_ctx* ctx, uint64_t* patch, uint64_t* short_sum, uint64_t* few_rows);
+
+/* ---- layers and updates the reference composes or lacks ----------------- */
+
+/* Layer normalisation: for each of `rows` rows of `cols` elements (row i at
+ * x + i * ldx, elements next to each other: a tensor normalised over its leading
+ * dims, dim 0 fastest)
+ *   m = mean(x)   r = 1 / sqrt(mean((x - m)^2) + eps)   y = (x - m) r weight + bias
+ * weight and bias have `cols` elements each; NULL stands for ones and zeros.
+ * mean / rstd: NULL, or `rows` elements each that receive m and r (what
+ * tcg_layer_norm_grad takes).  float and double; a row's sums are taken in the
+ * type of x, the mean with a correction for its own rounding.  A row of equal
+ * elements gives bias (with eps = 0: NaN, as the formula says); infinities and
+ * NaN stay in their row.  y may be x (same leading dim).  No rows: nothing is
+ * done.  The reference has no such operator: cfg/tenncor/core.yml composes it
+ * from reduce_mean, sub, square, sqrt and div. */
+int tcg_layer_norm (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols,
+	const void* x, uint64_t ldx, const void* weight, const void* bias, double eps,
+	void* y, uint64_t ldy, void* mean, void* rstd);
+/* The gradients of tcg_layer_norm for the gradient dy that arrives at y, with
+ * h = (x - m) r:
+ *   dx      = r (dy weight - mean(dy weight) - h mean(dy weight h))
+ *   dweight = sum over rows of dy h      dbias = sum over rows of dy
+ * Each of dx, dweight and dbias may be NULL (not all three); what is wanted
+ * together is computed in one pass over x and dy.  mean / rstd: what the forward
+ * pass left, or both NULL, and they are taken from x again (eps is used only
+ * then).  The sums over rows run in a fixed order: the same bits at every call.
+ * dx may be dy or x (same leading dim).  No rows: dweight and dbias are zero. */
+int tcg_layer_norm_grad (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols,
+	const void* dy, uint64_t lddy, const void* x, uint64_t ldx, const void* weight,
+	const void* mean, const void* rstd, double eps,
+	void* dx, uint64_t lddx, void* dweight, void* dbias);
 
 #ifdef __cplusplus
 }

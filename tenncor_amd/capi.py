@@ -31,6 +31,8 @@ OPCODES = [
     "STRIDE", "SCATTER", "POW", "ADD", "SUB", "MUL", "DIV", "MIN", "MAX", "EQ", "NEQ", "LT",
     "GT", "MATMUL", "CONTRACT", "CONV", "SELECT", "CONCAT", "ASSIGN", "ASSIGN_ADD",
     "ASSIGN_SUB", "ASSIGN_MUL", "ASSIGN_DIV", "CAST",
+    # nodes of this backend, behind those of cfg/ops.yml
+    "LAYER_NORM", "LAYER_NORM_DX", "LAYER_NORM_DWEIGHT",
 ]
 OP = {name: i for i, name in enumerate(OPCODES)}
 
@@ -47,6 +49,7 @@ EXPORTS = [
     "tcg_gemm", "tcg_gemm_terms", "tcg_gemm_terms_ranges", "tcg_gemm_terms_grid", "tcg_gemm_terms_fx", "tcg_jit_stats", "tcg_conv", "tcg_conv_boxed", "tcg_conv_dense_box", "tcg_conv_views", "tcg_conv_route_counts", "tcg_capture_begin", "tcg_capture_begin_small", "tcg_capture_feed", "tcg_graph_feed", "tcg_capture_end", "tcg_capture_abort", "tcg_batch_begin", "tcg_batch_end", "tcg_fork", "tcg_fork_end", "tcg_join",
     "tcg_graph_launch", "tcg_graph_claim", "tcg_graph_stats", "tcg_graph_destroy",
     "tcg_rand_seed", "tcg_rand_state", "tcg_rand_uniform",
+    "tcg_layer_norm", "tcg_layer_norm_grad",
 ]
 
 
@@ -86,7 +89,7 @@ def load():
         raise ImportError("%s is missing: build it with `python -m tenncor_amd.build` "
                           "(there is no CPU fallback)" % LIB_PATH)
     lib = ctypes.CDLL(LIB_PATH)
-    vp, u64, i32, sz = ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int, ctypes.c_size_t
+    vp, u64, i32, sz, f64 = ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int, ctypes.c_size_t, ctypes.c_double
     u64p, vpp = ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_void_p)
     i64p = ctypes.POINTER(ctypes.c_int64)
     sig = {
@@ -152,6 +155,8 @@ def load():
         "tcg_conv_dense_box": [vp, i32, u64p, u64p, i32, u64p, u64p, u64p, u64p, u64p, vp, vp, vp],
         "tcg_conv_views": [vp, i32, u64p, u64p, i32, u64p, u64p, u64p, u64p, u64p, vp, i64p, vp, i64p, vp, i64p],
         "tcg_conv_route_counts": [vp, u64p, u64p, u64p],
+        "tcg_layer_norm": [vp, i32, u64, u64, vp, u64, vp, vp, f64, vp, u64, vp, vp],
+        "tcg_layer_norm_grad": [vp, i32, u64, u64, vp, u64, vp, u64, vp, vp, vp, f64, vp, u64, vp, vp],
         "tcg_capture_begin": [vp],
         "tcg_capture_end": [vp, ctypes.POINTER(vp)],
         "tcg_capture_abort": [vp],
@@ -538,6 +543,19 @@ class Context:
         a, b, c = ctypes.c_uint64(), ctypes.c_uint64(), ctypes.c_uint64()
         self._check(self.lib.tcg_conv_route_counts(self.handle, ctypes.byref(a), ctypes.byref(b), ctypes.byref(c)))
         return {"patch": a.value, "short_sum": b.value, "few_rows": c.value}
+
+    # ---- layers and updates ----
+    def layer_norm(self, dtype, rows, cols, x, ldx, weight, bias, eps, y, ldy, mean=None, rstd=None):
+        """weight and bias: device addresses or None (ones, zeros); mean and rstd:
+        where the statistics of every row go, or None."""
+        self._check(self.lib.tcg_layer_norm(self.handle, dtype, rows, cols, x, ldx, weight, bias, eps, y, ldy, mean, rstd))
+
+    def layer_norm_grad(self, dtype, rows, cols, dy, lddy, x, ldx, weight, eps, dx=None, lddx=0, dweight=None, dbias=None,
+                        mean=None, rstd=None):
+        """Any of dx, dweight and dbias; mean and rstd as layer_norm left them, or
+        None to take them from x again."""
+        self._check(self.lib.tcg_layer_norm_grad(self.handle, dtype, rows, cols, dy, lddy, x, ldx, weight, mean, rstd, eps,
+                                                 dx, lddx, dweight, dbias))
 
     def jit_stats(self):
         """Kernels compiled at run time by this process, kernels loaded from the

@@ -140,6 +140,27 @@ int tcg_fail (tcg_ctx* ctx, int status, const char* fmt, ...);
 #define TCG_REQUIRE(ctx, cond, ...) do {\
 	if (!(cond)) { return tcg_fail(ctx, TCG_ERR_ARG, __VA_ARGS__); } } while (0)
 
+// The context's device is the current one for the life of this object: launches
+// and allocations of an entry point go there whatever the calling thread had set
+struct tcg_device_scope
+{
+	explicit tcg_device_scope (const tcg_ctx* ctx)
+	{
+		if (hipGetDevice(&before_) != hipSuccess) { before_ = ctx->device; }
+		if (before_ != ctx->device) { (void) hipSetDevice(ctx->device); }
+		now_ = ctx->device;
+	}
+	~tcg_device_scope (void)
+	{
+		if (before_ != now_) { (void) hipSetDevice(before_); }
+	}
+	tcg_device_scope (const tcg_device_scope&) = delete;
+	tcg_device_scope& operator = (const tcg_device_scope&) = delete;
+
+private:
+	int before_ = 0, now_ = 0;
+};
+
 static inline size_t tcg_type_size (int dtype)
 {
 	switch (dtype)

@@ -243,12 +243,15 @@ class Graph:
 
     # ---- functors ----
     def functor(self, op, args, **attrs):
-        """attrs: key -> list of ints (pairs flattened), a Node for `tensor`."""
+        """attrs: key -> list of ints (pairs flattened), a Node for `tensor`, a list
+        of numbers for `reals`."""
         opcode = OP[op] if isinstance(op, str) else int(op)
         keys, arrays = [], []
         for key, val in attrs.items():
             if isinstance(val, Node):
                 val = [val.id]
+            elif key == "reals":
+                val = [int(v) for v in np.asarray(val, np.float64).reshape(-1).view(np.int64)]
             elif np.isscalar(val):
                 val = [int(val)]
             keys.append(key.encode())
@@ -330,6 +333,8 @@ class Graph:
         self._check(self.lib.tcr_attr(self.h, node.id, key.encode(), buf, n.value, ctypes.byref(n)))
         if key == "tensor":
             return Node(self, int(buf[0]))
+        if key == "reals":
+            return [float(v) for v in np.array([buf[i] for i in range(n.value)], np.int64).view(np.float64)]
         return [int(buf[i]) for i in range(n.value)]
 
     def to_string(self, node):
@@ -535,6 +540,18 @@ class Api:
         shifted = self.sub(x, self.extend_like(self.reduce_max(x, offset, ndims), x))
         exarg = self.exp(shifted)
         return self.div(exarg, self.extend_like(self.add(self.reduce_sum(exarg, offset, ndims), eps), exarg))
+
+    def layer_norm(self, x, weight=None, bias=None, ndims=1, epsilon=1e-5):
+        """`x` normalised over its dims 0 .. ndims - 1, times weight plus bias (of
+        those dims' shape; without: ones and zeros).  One node; its gradients are
+        one for x, one for the weight and a REDUCE_SUM for the bias."""
+        args = [x] + ([weight] if weight is not None else [])
+        if bias is not None and weight is not None:
+            args.append(bias)
+        out = self.g.functor("LAYER_NORM", args, rank=ndims, reals=[epsilon])
+        if bias is not None and weight is None:
+            out = self.add(out, self.extend_like(bias, out))
+        return out
 
     def cross_entropy(self, target, x):
         """loss.yml:40-59."""

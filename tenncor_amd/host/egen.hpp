@@ -21,7 +21,11 @@ enum _GENERATED_OPCODE
 	REDUCE_MIN, REDUCE_MAX, ARGMAX, PERMUTE, EXTEND, RESHAPE, SLICE, PAD,
 	STRIDE, SCATTER, POW, ADD, SUB, MUL, DIV, MIN, MAX, EQ, NEQ, LT, GT,
 	MATMUL, CONTRACT, CONV, SELECT, CONCAT, ASSIGN, ASSIGN_ADD, ASSIGN_SUB,
-	ASSIGN_MUL, ASSIGN_DIV, CAST, _N_GENERATED_OPCODES
+	ASSIGN_MUL, ASSIGN_DIV, CAST,
+	// nodes of this backend, behind those of cfg/ops.yml so that the codes of
+	// stored graphs stay what they are
+	LAYER_NORM, LAYER_NORM_DX, LAYER_NORM_DWEIGHT,
+	_N_GENERATED_OPCODES
 };
 
 std::string name_op (_GENERATED_OPCODE code);

@@ -559,6 +559,78 @@ EigenptrT cast (const teq::TensptrT& input)
 	});
 }
 
+// ---- nodes of this backend (no counterpart in internal/eigen/operator.hpp) -------
+
+template <typename T>
+void need_real (const char* what)
+{
+	if (false == std::is_floating_point<T>::value) { global::fatalf("cannot %s integers", what); }
+}
+
+inline teq::CTensT const_args (const teq::TensptrsT& args)
+{
+	teq::CTensT out;
+	for (auto& arg : args) { out.push_back(arg.get()); }
+	return out;
+}
+
+/// A tensor normalised over its leading dims, as the matrix of the C ABI
+struct NormRows final
+{
+	NormRows (const teq::iTensor& x, const marsh::iAttributed& attrib)
+	{
+		teq::RankT rank;
+		Packer<teq::RankT>().unpack(rank, attrib);
+		RealsT reals;
+		Packer<RealsT>().unpack(reals, attrib);
+		eps = reals.at(0);
+		Shape8 shape = shape8(x.shape());
+		for (size_t i = 0; i < shape.size(); ++i) { (i < rank ? cols : rows) *= shape[i]; }
+	}
+
+	uint64_t rows = 1, cols = 1;
+	double eps = 0;
+};
+
+/// args: x, and perhaps weight, and perhaps bias
+template <typename T>
+EigenptrT layer_norm (teq::Shape outshape, const teq::TensptrsT& args, const marsh::iAttributed& attrib)
+{
+	need_real<T>("normalise");
+	NormRows n(*args[0], attrib);
+	return make_op<T>(outshape, const_args(args), [n](tcg_ctx* ctx, T* out, const std::vector<const void*>& args)
+	{
+		hip_check(tcg_layer_norm(ctx, egen::device_type<T>(), n.rows, n.cols, args[0], n.cols,
+			args.size() > 1 ? args[1] : nullptr, args.size() > 2 ? args[2] : nullptr, n.eps, out, n.cols, nullptr, nullptr));
+	});
+}
+
+/// args: the gradient that arrives, x, and perhaps weight
+template <typename T>
+EigenptrT layer_norm_dx (teq::Shape outshape, const teq::TensptrsT& args, const marsh::iAttributed& attrib)
+{
+	need_real<T>("normalise");
+	NormRows n(*args[1], attrib);
+	return make_op<T>(outshape, const_args(args), [n](tcg_ctx* ctx, T* out, const std::vector<const void*>& args)
+	{
+		hip_check(tcg_layer_norm_grad(ctx, egen::device_type<T>(), n.rows, n.cols, args[0], n.cols, args[1], n.cols,
+			args.size() > 2 ? args[2] : nullptr, nullptr, nullptr, n.eps, out, n.cols, nullptr, nullptr));
+	});
+}
+
+/// args: the gradient that arrives, x
+template <typename T>
+EigenptrT layer_norm_dweight (teq::Shape outshape, const teq::TensptrsT& args, const marsh::iAttributed& attrib)
+{
+	need_real<T>("normalise");
+	NormRows n(*args[1], attrib);
+	return make_op<T>(outshape, const_args(args), [n](tcg_ctx* ctx, T* out, const std::vector<const void*>& args)
+	{
+		hip_check(tcg_layer_norm_grad(ctx, egen::device_type<T>(), n.rows, n.cols, args[0], n.cols, args[1], n.cols,
+			nullptr, nullptr, nullptr, n.eps, nullptr, 0, out, nullptr));
+	});
+}
+
 }
 
 namespace egen
@@ -630,6 +702,9 @@ void typed_exec (_GENERATED_OPCODE opcode, eigen::EigenptrT& out, teq::Shape out
 		case ASSIGN_MUL: need(2); out = eigen::assign_mul<T>(*in[0], *in[1]); break;
 		case ASSIGN_DIV: need(2); out = eigen::assign_div<T>(*in[0], *in[1]); break;
 		case CAST: out = eigen::cast<T>(in[0]); break;
+		case LAYER_NORM: out = eigen::layer_norm<T>(outshape, in, attrib); break;
+		case LAYER_NORM_DX: need(2); out = eigen::layer_norm_dx<T>(outshape, in, attrib); break;
+		case LAYER_NORM_DWEIGHT: need(2); out = eigen::layer_norm_dweight<T>(outshape, in, attrib); break;
 		default: global::fatal("unknown opcode");
 	}
 }
@@ -652,7 +727,8 @@ void typed_exec (_GENERATED_OPCODE opcode, eigen::EigenptrT& out, teq::Shape out
 	TCH_OP_CASE(MACRO, MATMUL) TCH_OP_CASE(MACRO, CONTRACT) TCH_OP_CASE(MACRO, CONV) TCH_OP_CASE(MACRO, SELECT)\
 	TCH_OP_CASE(MACRO, CONCAT) TCH_OP_CASE(MACRO, ASSIGN) TCH_OP_CASE(MACRO, ASSIGN_ADD)\
 	TCH_OP_CASE(MACRO, ASSIGN_SUB) TCH_OP_CASE(MACRO, ASSIGN_MUL) TCH_OP_CASE(MACRO, ASSIGN_DIV)\
-	TCH_OP_CASE(MACRO, CAST) default: global::fatal("executing bad op"); }
+	TCH_OP_CASE(MACRO, CAST) TCH_OP_CASE(MACRO, LAYER_NORM) TCH_OP_CASE(MACRO, LAYER_NORM_DX)\
+	TCH_OP_CASE(MACRO, LAYER_NORM_DWEIGHT) default: global::fatal("executing bad op"); }
 
 }
 

@@ -1,4 +1,4 @@
-// Attribute packers: the nine keys and encodings of tenncor's
+// Attribute packers (one of them, `reals`, this backend's own): the nine keys and encodings of tenncor's
 // internal/eigen/packattr.hpp:60-363 (every numeric list is a
 // NumArray<int64_t>, pairs are flattened, `rank` is a Number<int64_t>, `dtype`
 // is the type's name, `tensor` holds the node itself) and unpack_extend of
@@ -263,6 +263,29 @@ struct Packer<teq::TensptrT>
 		auto obj = dynamic_cast<const teq::TensorObj*>(get_attr(*this, attrib));
 		if (nullptr == obj) { global::fatal("`tensor` attribute does not hold a tensor"); }
 		out = obj->get_tensor();
+	}
+};
+
+/// Real parameters of an operator.  Held as the bits of the doubles, so that two
+/// nodes are told apart by every bit of theirs (attributes are compared and
+/// labelled as integers) and integer bindings can pass them on
+using RealsT = std::vector<double>;
+
+template <>
+struct Packer<RealsT>
+{
+	std::string get_key (void) const { return "reals"; }
+	void pack (marsh::iAttributed& attrib, RealsT reals) const
+	{
+		std::vector<int64_t> bits(reals.size());
+		for (size_t i = 0; i < reals.size(); ++i) { memcpy(&bits[i], &reals[i], sizeof(double)); }
+		attrib.add_attr(get_key(), std::make_unique<marsh::NumArray<int64_t>>(bits));
+	}
+	void unpack (RealsT& out, const marsh::iAttributed& attrib) const
+	{
+		auto& bits = int_contents(get_attr(*this, attrib));
+		out.resize(bits.size());
+		for (size_t i = 0; i < bits.size(); ++i) { memcpy(&out[i], &bits[i], sizeof(double)); }
 	}
 };
 

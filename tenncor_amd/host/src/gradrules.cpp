@@ -359,6 +359,22 @@ Node rule_select (const Site& s)
 	return 1 == s.k ? make(egen::SELECT, {s.in[0], s.up, nothing}) : make(egen::SELECT, {s.in[0], nothing, s.up});
 }
 
+// LAYER_NORM(x, weight, bias): two nodes of their own, and the sum over the rows for the bias
+Node rule_layer_norm (const Site& s)
+{
+	auto rank = s.attr<teq::RankT>();
+	if (2 == s.k)
+	{
+		std::set<teq::RankT> rows;
+		for (teq::RankT d = rank; d < teq::rank_cap; ++d) { rows.emplace(d); }
+		return make(egen::REDUCE_SUM, {s.up}, rows);
+	}
+	auto reals = s.attr<eigen::RealsT>();
+	if (1 == s.k) { return make(egen::LAYER_NORM_DWEIGHT, {s.up, s.x()}, rank, reals); }
+	if (1 == s.in.size()) { return make(egen::LAYER_NORM_DX, {s.up, s.x()}, rank, reals); }
+	return make(egen::LAYER_NORM_DX, {s.up, s.x(), s.in[1]}, rank, reals);
+}
+
 Node rule_zero (const Site& s) { return filled(0.f, s.x()); }
 
 Node rule_refused (const Site& s)
@@ -407,9 +423,10 @@ const std::vector<Rule>& rule_table (void)
 		t[egen::SCATTER] = rule_scatter;
 		t[egen::REVERSE] = rule_reverse;
 		t[egen::SELECT] = rule_select;
+		t[egen::LAYER_NORM] = rule_layer_norm;
 		for (auto code : {egen::RAND_UNIF, egen::EQ, egen::NEQ, egen::GT, egen::LT}) { t[code] = rule_zero; }
 		for (auto code : {egen::ASSIGN, egen::ASSIGN_ADD, egen::ASSIGN_SUB, egen::ASSIGN_MUL, egen::ASSIGN_DIV,
-			egen::ARGMAX}) { t[code] = rule_refused; }
+			egen::ARGMAX, egen::LAYER_NORM_DX, egen::LAYER_NORM_DWEIGHT}) { t[code] = rule_refused; }
 		return t;
 	}();
 	return table;

@@ -13,6 +13,7 @@ static const char* opnames[] = {
 	"STRIDE", "SCATTER", "POW", "ADD", "SUB", "MUL", "DIV", "MIN", "MAX", "EQ", "NEQ", "LT",
 	"GT", "MATMUL", "CONTRACT", "CONV", "SELECT", "CONCAT", "ASSIGN", "ASSIGN_ADD",
 	"ASSIGN_SUB", "ASSIGN_MUL", "ASSIGN_DIV", "CAST",
+	"LAYER_NORM", "LAYER_NORM_DX", "LAYER_NORM_DWEIGHT",
 };
 
 std::string name_op (_GENERATED_OPCODE code)
@@ -68,6 +69,40 @@ static teq::Shape same_shape (_GENERATED_OPCODE opcode, const teq::ShapesT& shap
 		}
 	}
 	return outshape;
+}
+
+/// The dims LAYER_NORM and its gradients normalise over: 0 .. rank - 1
+static teq::RankT norm_rank (_GENERATED_OPCODE opcode, const marsh::Maps& attrs)
+{
+	teq::RankT rank;
+	eigen::Packer<teq::RankT>().unpack(rank, attrs);
+	if (0 == rank || rank >= teq::rank_cap)
+	{
+		global::throw_errf("cannot %s over %d dims: 1 to %d are possible", name_op(opcode).c_str(),
+			(int) rank, (int) teq::rank_cap - 1);
+	}
+	eigen::RealsT reals;
+	eigen::Packer<eigen::RealsT>().unpack(reals, attrs);
+	if (reals.size() != 1 || false == (reals[0] >= 0))
+	{
+		global::throw_errf("cannot %s without one epsilon that is not negative", name_op(opcode).c_str());
+	}
+	return rank;
+}
+
+/// The shape of a weight: the dims that are normalised over, then ones
+static teq::Shape norm_weight_shape (teq::Shape shape, teq::RankT rank)
+{
+	return teq::Shape(teq::DimsT(shape.begin(), shape.begin() + rank));
+}
+
+static void need_norm_weight (_GENERATED_OPCODE opcode, teq::Shape shape, teq::RankT rank, teq::Shape weight)
+{
+	if (false == norm_weight_shape(shape, rank).compatible_after(weight, 0))
+	{
+		global::throw_errf("cannot %s shape %s over %d dims with a weight or bias of shape %s", name_op(opcode).c_str(),
+			shape.to_string().c_str(), (int) rank, weight.to_string().c_str());
+	}
 }
 
 teq::Shape parse_shape (_GENERATED_OPCODE opcode, const marsh::Maps& attrs, const teq::ShapesT& shapes)
@@ -321,6 +356,26 @@ teq::Shape parse_shape (_GENERATED_OPCODE opcode, const marsh::Maps& attrs, cons
 			}
 			return teq::Shape(slist);
 		}
+		case LAYER_NORM: // x, and perhaps weight, and perhaps bias
+		{
+			need_args(shapes);
+			teq::RankT rank = norm_rank(opcode, attrs);
+			if (shapes.size() > 3) { global::throw_errf("cannot %s with %d arguments", name_op(opcode).c_str(), (int) shapes.size()); }
+			for (size_t i = 1; i < shapes.size(); ++i) { need_norm_weight(opcode, shapes.front(), rank, shapes[i]); }
+			return shapes.front();
+		}
+		case LAYER_NORM_DX: // the arriving gradient, x, and perhaps weight
+		case LAYER_NORM_DWEIGHT: // the arriving gradient, x
+		{
+			teq::RankT rank = norm_rank(opcode, attrs);
+			if (shapes.size() < 2 || shapes.size() > (LAYER_NORM_DX == opcode ? 3 : 2))
+			{
+				global::throw_errf("cannot %s with %d arguments", name_op(opcode).c_str(), (int) shapes.size());
+			}
+			(void) same_shape(opcode, {shapes[0], shapes[1]});
+			if (shapes.size() > 2) { need_norm_weight(opcode, shapes[1], rank, shapes[2]); }
+			return LAYER_NORM_DX == opcode ? shapes[1] : norm_weight_shape(shapes[1], rank);
+		}
 		case ASSIGN: case ASSIGN_ADD: case ASSIGN_SUB: case ASSIGN_MUL: case ASSIGN_DIV:
 		default:
 			return same_shape(opcode, shapes);
@@ -342,9 +397,16 @@ _GENERATED_DTYPE parse_type (_GENERATED_OPCODE opcode, const marsh::Maps& attrs,
 				return out;
 			}
 			return dtypes.front();
-		default: // :52-62
-			return *std::max_element(dtypes.begin(), dtypes.end(),
+		default: // :52-62; this backend's own nodes (behind CAST) are for real types
+		{
+			_GENERATED_DTYPE out = *std::max_element(dtypes.begin(), dtypes.end(),
 				[](_GENERATED_DTYPE lhs, _GENERATED_DTYPE rhs) { return type_precision(lhs) < type_precision(rhs); });
+			if (opcode > CAST && DOUBLE != out && FLOAT != out)
+			{
+				global::throw_errf("cannot %s integers", name_op(opcode).c_str());
+			}
+			return out;
+		}
 	}
 }
 

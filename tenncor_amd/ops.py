@@ -110,6 +110,46 @@ def argmax(x, return_dim):
     return out
 
 
+def _norm_rows(x, ndims):
+    if not 1 <= ndims <= RANK_CAP:
+        raise ValueError("cannot normalise shape %s over %d dims" % (x.shape, ndims))
+    cols = capi.n_elems(x.shape[:ndims])
+    return x.n // cols if cols else 0, cols
+
+
+def _norm_weight(x, ndims, *params):
+    for p in params:
+        if p is not None and p.shape != capi.shape8(x.shape[:ndims]):
+            raise ValueError("cannot normalise shape %s over %d dims with a weight or bias of shape %s" % (x.shape, ndims, p.shape))
+        if p is not None and p.dtype != x.dtype:
+            raise ValueError("weight, bias and tensor are of one type")
+
+
+def layer_norm(x, weight=None, bias=None, ndims=1, epsilon=1e-5, stats=False):
+    """`x` normalised over its dims 0 .. ndims - 1.  stats: (result, mean, rstd) with
+    one element of the last two for every row."""
+    _norm_weight(x, ndims, weight, bias)
+    rows, cols = _norm_rows(x, ndims)
+    out = _new(x.ctx, x.shape, x)
+    kept = [_new(x.ctx, [1] * ndims + x.shape[ndims:], x) for _ in range(2)] if stats else [None, None]
+    x.ctx.layer_norm(x.dtype, rows, cols, x.ptr, cols, weight and weight.ptr, bias and bias.ptr, epsilon, out.ptr, cols,
+                     *[k and k.ptr for k in kept])
+    return (out, *kept) if stats else out
+
+
+def layer_norm_grad(up, x, weight=None, ndims=1, epsilon=1e-5, mean=None, rstd=None):
+    """(dx, dweight, dbias) for the gradient `up` that arrives at layer_norm(x, ...)."""
+    _same_shape("LAYER_NORM_DX", [up, x])
+    _norm_weight(x, ndims, weight)
+    rows, cols = _norm_rows(x, ndims)
+    dx = _new(x.ctx, x.shape, x)
+    dweight, dbias = (_new(x.ctx, x.shape[:ndims], x) for _ in range(2))
+    x.ctx.layer_norm_grad(x.dtype, rows, cols, up.ptr, cols, x.ptr, cols, weight and weight.ptr, epsilon,
+                          dx=dx.ptr, lddx=cols, dweight=dweight.ptr, dbias=dbias.ptr,
+                          mean=mean and mean.ptr, rstd=rstd and rstd.ptr)
+    return dx, dweight, dbias
+
+
 def extend(x, bcast):
     """cfg/ops.yml:256-283."""
     b = capi.shape8(bcast)
