@@ -92,7 +92,8 @@ enum tcg_opcode
 	TCG_ASSIGN, TCG_ASSIGN_ADD, TCG_ASSIGN_SUB, TCG_ASSIGN_MUL, TCG_ASSIGN_DIV,
 	TCG_CAST,
 	/* nodes of this backend's graphs that cfg/ops.yml does not have */
-	TCG_LAYER_NORM, TCG_LAYER_NORM_DX, TCG_LAYER_NORM_DWEIGHT, TCG_N_OPCODES
+	TCG_LAYER_NORM, TCG_LAYER_NORM_DX, TCG_LAYER_NORM_DWEIGHT,
+	TCG_ORTHOGONALIZE, TCG_N_OPCODES
 };
 
 /* ---- context, memory, transfers -------------------------------------- */
@@ -680,6 +681,25 @@ int tcg_layer_norm_grad (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols,
 	const void* dy, uint64_t lddy, const void* x, uint64_t ldx, const void* weight,
 	const void* mean, const void* rstd, double eps,
 	void* dx, uint64_t lddx, void* dweight, void* dbias);
+
+/* The orthogonalised update of weight matrices: `batch` matrices of rows x cols
+ * elements (matrix z, row i at in + z * stride_i + i * ldi), each by itself
+ *   X = G / (|G| + eps), |G| the root of the sum of its squares,
+ *   A = X X^T    B = coef[1] A + coef[2] A A    X <- coef[0] X + B X
+ * `steps` times (with the transposed of X where rows > cols, which gives the
+ * same): every singular value s of X becomes coef[0] s + coef[1] s^3 + coef[2] s^5
+ * at each step while its singular vectors stay, and with coefficients that drive
+ * the values towards one the result is near the closest orthogonal matrix.  A
+ * matrix of zeros stays one (eps > 0); a NaN or an infinity makes its whole matrix
+ * NaN and leaves the others alone.
+ * float and double.  In float the products run on half-precision matrix
+ * instructions with every operand as two halves (22 bits and more of each value)
+ * and sums in fp32: results are as near to the formulas as with fp32 products.
+ * 1 to 64 steps; coefficients under which values of up to one grow past 1e6 are
+ * refused.  out may be in, laid out alike.  The reference has no such operator. */
+int tcg_orthogonalize (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols, uint64_t batch,
+	const void* in, uint64_t ldi, uint64_t stride_i, int steps, const double coef[3], double eps,
+	void* out, uint64_t ldo, uint64_t stride_o);
 
 #ifdef __cplusplus
 }

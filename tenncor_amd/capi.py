@@ -32,7 +32,7 @@ OPCODES = [
     "GT", "MATMUL", "CONTRACT", "CONV", "SELECT", "CONCAT", "ASSIGN", "ASSIGN_ADD",
     "ASSIGN_SUB", "ASSIGN_MUL", "ASSIGN_DIV", "CAST",
     # nodes of this backend, behind those of cfg/ops.yml
-    "LAYER_NORM", "LAYER_NORM_DX", "LAYER_NORM_DWEIGHT",
+    "LAYER_NORM", "LAYER_NORM_DX", "LAYER_NORM_DWEIGHT", "ORTHOGONALIZE",
 ]
 OP = {name: i for i, name in enumerate(OPCODES)}
 
@@ -49,7 +49,7 @@ EXPORTS = [
     "tcg_gemm", "tcg_gemm_terms", "tcg_gemm_terms_ranges", "tcg_gemm_terms_grid", "tcg_gemm_terms_fx", "tcg_jit_stats", "tcg_conv", "tcg_conv_boxed", "tcg_conv_dense_box", "tcg_conv_views", "tcg_conv_route_counts", "tcg_capture_begin", "tcg_capture_begin_small", "tcg_capture_feed", "tcg_graph_feed", "tcg_capture_end", "tcg_capture_abort", "tcg_batch_begin", "tcg_batch_end", "tcg_fork", "tcg_fork_end", "tcg_join",
     "tcg_graph_launch", "tcg_graph_claim", "tcg_graph_stats", "tcg_graph_destroy",
     "tcg_rand_seed", "tcg_rand_state", "tcg_rand_uniform",
-    "tcg_layer_norm", "tcg_layer_norm_grad",
+    "tcg_layer_norm", "tcg_layer_norm_grad", "tcg_orthogonalize",
 ]
 
 
@@ -156,6 +156,7 @@ def load():
         "tcg_conv_views": [vp, i32, u64p, u64p, i32, u64p, u64p, u64p, u64p, u64p, vp, i64p, vp, i64p, vp, i64p],
         "tcg_conv_route_counts": [vp, u64p, u64p, u64p],
         "tcg_layer_norm": [vp, i32, u64, u64, vp, u64, vp, vp, f64, vp, u64, vp, vp],
+        "tcg_orthogonalize": [vp, i32, u64, u64, u64, vp, u64, u64, i32, ctypes.POINTER(f64), f64, vp, u64, u64],
         "tcg_layer_norm_grad": [vp, i32, u64, u64, vp, u64, vp, u64, vp, vp, vp, f64, vp, u64, vp, vp],
         "tcg_capture_begin": [vp],
         "tcg_capture_end": [vp, ctypes.POINTER(vp)],
@@ -556,6 +557,13 @@ class Context:
         None to take them from x again."""
         self._check(self.lib.tcg_layer_norm_grad(self.handle, dtype, rows, cols, dy, lddy, x, ldx, weight, mean, rstd, eps,
                                                  dx, lddx, dweight, dbias))
+
+    def orthogonalize(self, dtype, rows, cols, batch, src, ldi, stride_i, dst, ldo, stride_o, steps=5,
+                      coef=(3.4445, -4.7750, 2.0315), eps=1e-7):
+        """The default coefficients take every singular value above 1e-2 of the norm to
+        between 0.68 and 1.13 in five steps."""
+        self._check(self.lib.tcg_orthogonalize(self.handle, dtype, rows, cols, batch, src, ldi, stride_i, steps,
+                                               (ctypes.c_double * 3)(*coef), eps, dst, ldo, stride_o))
 
     def jit_stats(self):
         """Kernels compiled at run time by this process, kernels loaded from the

@@ -1,0 +1,779 @@
+// The orthogonalised update of a weight matrix (the step of a momentum matrix G
+// along its singular directions): with an odd polynomial p(s) = a s + b s^3 + c s^5
+// and X = G / (|G| + eps), transposed when it has more rows than columns,
+//
+//   A = X X^T      B = b A + c A A      X <- a X + B X       `steps` times
+//
+// which applies p to every singular value of X and leaves its singular vectors.
+// With m rows and n >= m columns a step is m^2 n + m^3 + 2 m^2 n multiplications
+// and additions (one triangle of the symmetric A and A A): bound by the matrix
+// instructions.
+//
+// fp32: an operand of a product is two halves of 16 bits, x s = hi + lo with
+// hi = half(x s), lo = half(x s - hi) and a power of two s that puts the largest
+// value the matrix can hold (the host follows the polynomial from |x| <= 1) at
+// 2^15.  Each conversion is off by 2^-11 of what it converts at most, so 2^-22 of
+// the value is lost in the worst case.  A product is hi hi + hi lo + lo hi with the
+// sums in fp32; lo lo would be 2^-22 of the product.  Three half-precision matrix
+// instructions (2.5 PFLOP/s / 3) stand for one fp32 instruction (0.157 PFLOP/s),
+// and one load of hi and lo feeds three of them.
+//
+// What an error of X does is multiplied by up to a in each later step along the
+// weak directions of G, while one of A is read through B, which is small against
+// a there.  So a X is taken from X in fp32, and the sums of B X are cut every 256
+// indices and the parts added up apart: with both, results are as near to the
+// formulas as with fp32 products (1.6e-6 of the result's norm at 512 x 768; with
+// a X from the halves 3.2e-6, with uncut sums over 4096 indices 1e-5 and more).
+//
+// double: the same steps through the products of tcg_gemm.
+#include "tcg_internal.hpp"
+
+#include <cmath>
+#include <new>
+
+namespace
+{
+
+typedef _Float16 f16;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+
+// A row of a split matrix: for every 32 elements 32 hi and then 32 lo, 128 bytes
+constexpr uint32_t BLOCK = 64; // halves
+constexpr uint32_t FLUSH = 8;  // slabs of 32 summed indices between two cuts of the sums of B X
+
+struct Split
+{
+	f16 hi, lo;
+};
+
+__device__ __forceinline__ Split split (float v)
+{
+	Split s;
+	s.hi = (f16) v;
+	s.lo = (f16) (v - (float) s.hi);
+	return s;
+}
+
+// ---- the norm, and the first split -------------------------------------------------
+
+constexpr uint32_t NORM_PARTS = 256; // workgroups that sum one matrix at most
+
+template <typename T>
+struct PrepArgs
+{
+	const T* g;
+	uint64_t ldg, stride_g;
+	uint64_t rows, cols;
+	uint32_t parts;
+	double* sums; // [batch][parts]
+	double eps;
+	float scale;
+	// float: X and X^T as split matrices, mp x np padded; double: X dense
+	f16* x;
+	f16* xt;
+	uint64_t ldx, stride_x, ldxt, stride_xt;
+	float* xt32; // X^T in fp32, rows of ldxt / 2
+	T* dense;
+	uint64_t stride_dense;
+	bool tall; // X = G^T
+};
+
+__device__ __forceinline__ double group_sum (double v, double* red)
+{
+#pragma unroll
+	for (int d = TCG_WAVE / 2; d > 0; d >>= 1) { v += __shfl_xor(v, d); }
+	if ((threadIdx.x & (TCG_WAVE - 1)) == 0) { red[threadIdx.x / TCG_WAVE] = v; }
+	__syncthreads();
+	double out = 0;
+	for (uint32_t w = 0; w < blockDim.x / TCG_WAVE; ++w) { out += red[w]; }
+	__syncthreads();
+	return out;
+}
+
+// Sums of squares in double: an error of the norm is one of every singular value
+template <typename T>
+__global__ __launch_bounds__(256) void ortho_norm_k (PrepArgs<T> a)
+{
+	__shared__ double red[4];
+	const T* g = a.g + blockIdx.y * a.stride_g;
+	double sum = 0;
+	// rows dealt to the workgroups' waves, lanes along a row
+	const uint32_t wave = threadIdx.x / TCG_WAVE, lane = threadIdx.x & (TCG_WAVE - 1);
+	for (uint64_t row = (uint64_t) blockIdx.x * 4 + wave; row < a.rows; row += (uint64_t) a.parts * 4)
+	{
+		const T* p = g + row * a.ldg;
+#pragma unroll 4
+		for (uint64_t col = lane; col < a.cols; col += TCG_WAVE)
+		{
+			const double v = p[col];
+			sum += v * v;
+		}
+	}
+	sum = group_sum(sum, red);
+	if (threadIdx.x == 0) { a.sums[(uint64_t) blockIdx.y * a.parts + blockIdx.x] = sum; }
+}
+
+/// 1 / (|G| + eps) in every lane
+template <typename T>
+__device__ __forceinline__ double inverse_norm (const PrepArgs<T>& a, uint32_t batch, double* red)
+{
+	double sum = 0;
+	for (uint32_t p = threadIdx.x; p < a.parts; p += blockDim.x) { sum += a.sums[(uint64_t) batch * a.parts + p]; }
+	return 1. / (::sqrt(group_sum(sum, red)) + a.eps);
+}
+
+// X = G / (|G| + eps) and X^T as split matrices, a 64 x 64 tile a workgroup; what
+// lies outside G is zero
+__global__ __launch_bounds__(256) void ortho_split_k (PrepArgs<float> a, uint32_t tiles_x)
+{
+	__shared__ double red[4];
+	__shared__ float tile[64][65];
+	const uint32_t batch = blockIdx.y;
+	const double inv = inverse_norm(a, batch, red) * a.scale;
+	const uint64_t r0 = (uint64_t) (blockIdx.x / tiles_x) * 64, c0 = (uint64_t) (blockIdx.x % tiles_x) * 64;
+	const float* g = a.g + batch * a.stride_g;
+	for (uint32_t e = threadIdx.x; e < 64 * 64; e += 256)
+	{
+		const uint32_t r = e / 64, c = e % 64;
+		float v = 0;
+		if (r0 + r < a.rows && c0 + c < a.cols) { v = (float) ((double) g[(r0 + r) * a.ldg + c0 + c] * inv); }
+		tile[r][c] = v;
+	}
+	__syncthreads();
+	// G's rows are X's rows, or X^T's
+	f16* along = (a.tall ? a.xt + batch * a.stride_xt : a.x + batch * a.stride_x);
+	f16* across = (a.tall ? a.x + batch * a.stride_x : a.xt + batch * a.stride_xt);
+	const uint64_t ld_along = a.tall ? a.ldxt : a.ldx, ld_across = a.tall ? a.ldx : a.ldxt;
+	for (uint32_t e = threadIdx.x; e < 64 * 16; e += 256)
+	{
+		const uint32_t r = e / 16, c = e % 16 * 4;
+		f16x4 hi, lo, thi, tlo;
+#pragma unroll
+		for (int i = 0; i < 4; ++i)
+		{
+			const Split s = split(tile[r][c + i]), t = split(tile[c + i][r]);
+			hi[i] = s.hi; lo[i] = s.lo;
+			thi[i] = t.hi; tlo[i] = t.lo;
+		}
+		f16* p = along + (r0 + r) * ld_along + (c0 + c) / 32 * BLOCK + c % 32;
+		*reinterpret_cast<f16x4*>(p) = hi;
+		*reinterpret_cast<f16x4*>(p + 32) = lo;
+		f16* q = across + (c0 + r) * ld_across + (r0 + c) / 32 * BLOCK + c % 32;
+		*reinterpret_cast<f16x4*>(q) = thi;
+		*reinterpret_cast<f16x4*>(q + 32) = tlo;
+		float4 wide;
+		uint64_t row, col;
+		if (a.tall)
+		{
+			wide = make_float4(tile[r][c], tile[r][c + 1], tile[r][c + 2], tile[r][c + 3]);
+			row = r0 + r; col = c0 + c;
+		}
+		else
+		{
+			wide = make_float4(tile[c][r], tile[c + 1][r], tile[c + 2][r], tile[c + 3][r]);
+			row = c0 + r; col = r0 + c;
+		}
+		*reinterpret_cast<float4*>(a.xt32 + batch * (a.stride_xt / 2) + row * (a.ldxt / 2) + col) = wide;
+	}
+}
+
+// ---- the products over split matrices ------------------------------------------------
+
+enum Product
+{
+	GRAM = 0, // A = X X^T
+	FACTOR,   // B = b A + c A A
+	APPLY,    // X <- a X + B X, X^T along with it
+	LAST      // the same into the caller's matrix
+};
+
+struct PairArgs
+{
+	// C(i, j) = sum_k P(i, k) Q(j, k): rows of two split matrices
+	const f16* p;
+	const f16* q;
+	uint64_t ldp, ldq, stride_p, stride_q;
+	uint32_t slabs; // of 32 summed indices
+	uint32_t tiles_m, tiles_n, tiles; // tiles: of one matrix (one triangle of them for GRAM and FACTOR)
+	// C alpha + add beta; row j of `add` holds what meets C(., j): the split matrix A
+	// (FACTOR), or X^T in fp32
+	const f16* add;
+	const float* add32;
+	uint64_t ldadd, stride_add; // in elements of the one that is given
+	float alpha, beta;
+	// the result: row i, and row j of its transposed
+	f16* out;
+	f16* out_t;
+	float* out_t32; // APPLY: X^T in fp32, laid out like add32
+	uint64_t ldo, ldot, stride_o, stride_ot;
+	// LAST
+	float* last;
+	uint64_t ldl, stride_l;
+	uint32_t m, n;
+	bool tall;
+};
+
+/// Which 16 bytes of a row's 128 lie in which place in LDS: rows whose chunks a
+/// load of a matrix operand reads together never share banks
+__device__ __forceinline__ uint32_t swizzle (uint32_t row) { return ((row >> 1) & 7) ^ ((row & 1) << 2); }
+
+// WT: 32 x 32 blocks along each side of a wave's tile; four waves 2 x 2.  SLABS of
+// 32 summed indices have room in LDS: one is multiplied while SLABS - 1 are on
+// their way.
+template <int WT, int SLABS>
+constexpr int pair_lds = SLABS * 2 * 64 * WT * 128;
+
+template <int WT, int SLABS, int MODE>
+__global__ __launch_bounds__(256, 2) void ortho_pair_k (PairArgs g)
+{
+	constexpr int TILE = 64 * WT;
+	constexpr int OPERAND = TILE * 128; // bytes of an operand's slab in LDS
+	constexpr int LOADS = 2 * WT;       // a wave's loads per operand and slab
+	constexpr bool SYMMETRIC = MODE == GRAM || MODE == FACTOR;
+	constexpr bool CUT = MODE == APPLY || MODE == LAST;
+	static_assert(pair_lds<WT,SLABS> >= 4 * 4 * (32 * WT) * (32 * WT), "the result's way through LDS");
+	extern __shared__ __attribute__((aligned(1024))) char lds[];
+
+	// consecutive workgroups go to the XCDs in turn: each XCD gets a run of
+	// neighbouring tiles, which share rows of P
+	const uint32_t total = gridDim.x, xcd = blockIdx.x % 8, each = total / 8, more = total % 8;
+	const uint32_t at = xcd * each + (xcd < more ? xcd : more) + blockIdx.x / 8;
+	const uint32_t batch = at / g.tiles;
+	const uint32_t tile = at % g.tiles;
+	uint32_t bi, bj;
+	if constexpr (SYMMETRIC)
+	{
+		bi = (uint32_t) ((sqrtf(8.f * (float) tile + 1.f) - 1.f) * 0.5f);
+		while (bi * (bi + 1) / 2 > tile) { --bi; }
+		while ((bi + 1) * (bi + 2) / 2 <= tile) { ++bi; }
+		bj = tile - bi * (bi + 1) / 2;
+	}
+	else
+	{
+		bi = tile % g.tiles_m;
+		bj = tile / g.tiles_m;
+	}
+	const uint32_t wave = threadIdx.x / TCG_WAVE, lane = threadIdx.x & (TCG_WAVE - 1);
+	const uint32_t wi = wave / 2, wj = wave % 2, l32 = lane & 31, half = lane >> 5;
+
+	// where a lane's loads start: 8 rows a load, 8 lanes a row
+	const f16* from[2][LOADS];
+	uint32_t to[2][LOADS];
+#pragma unroll
+	for (int i = 0; i < LOADS; ++i)
+	{
+		const uint32_t r = wave * (16 * WT) + i * 8 + lane / 8;
+		const uint32_t chunk = (lane & 7) ^ swizzle(r);
+		from[0][i] = g.p + batch * g.stride_p + ((uint64_t) bi * TILE + r) * g.ldp + chunk * 8;
+		from[1][i] = g.q + batch * g.stride_q + ((uint64_t) bj * TILE + r) * g.ldq + chunk * 8;
+		const uint32_t base = (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) char*) lds + (wave * (16 * WT) + i * 8) * 128;
+		to[0][i] = __builtin_amdgcn_readfirstlane(base);
+		to[1][i] = __builtin_amdgcn_readfirstlane(base + OPERAND);
+	}
+	uint32_t ahead = BLOCK;
+	// the next slab of both operands into LDS buffer `b`, 16 bytes a lane straight from memory.
+	// The instruction itself: for its builtin the compiler waits for every such load
+	// before any later read of LDS.  The s_nop is the wait state between the write of M0
+	// and its use.
+	auto issue = [&] (uint32_t b)
+	{
+#pragma unroll
+		for (int o = 0; o < 2; ++o)
+		{
+#pragma unroll
+			for (int i = 0; i < LOADS; ++i)
+			{
+				asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+					: : "v"(from[o][i]), "s"(to[o][i] + b * 2 * OPERAND) : "memory", "m0");
+				from[o][i] += ahead;
+			}
+		}
+	};
+	f32x16 acc[WT][WT] = {}, sum[WT][WT] = {};
+	auto multiply = [&] (uint32_t b)
+	{
+		const char* P = lds + b * 2 * OPERAND;
+		const char* Q = P + OPERAND;
+#pragma unroll
+		for (int s = 0; s < 2; ++s)
+		{
+			f16x8 ph[WT], pl[WT], qh[WT], ql[WT];
+#pragma unroll
+			for (int t = 0; t < WT; ++t)
+			{
+				const uint32_t rp = wi * (32 * WT) + t * 32 + l32, rq = wj * (32 * WT) + t * 32 + l32;
+				const uint32_t c = 2 * s + half, fp = swizzle(rp), fq = swizzle(rq);
+				ph[t] = *reinterpret_cast<const f16x8*>(P + rp * 128 + (c ^ fp) * 16);
+				pl[t] = *reinterpret_cast<const f16x8*>(P + rp * 128 + ((c + 4) ^ fp) * 16);
+				qh[t] = *reinterpret_cast<const f16x8*>(Q + rq * 128 + (c ^ fq) * 16);
+				ql[t] = *reinterpret_cast<const f16x8*>(Q + rq * 128 + ((c + 4) ^ fq) * 16);
+			}
+#pragma unroll
+			for (int i = 0; i < WT; ++i)
+			{
+#pragma unroll
+				for (int j = 0; j < WT; ++j)
+				{
+					acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
+					acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
+					acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
+				}
+			}
+		}
+	};
+	// Every step issues the loads of one slab (past the end none is left: the last
+	// one again, never used), so with the loads of SLABS - 2 slabs out the slab
+	// of the step has landed: loads complete in order.  Behind the barrier every wave
+	// is done with the buffer that the step's loads overwrite.
+	auto landed = [] ()
+	{
+		constexpr int OUT = (SLABS - 2) * 2 * LOADS;
+		static_assert(OUT < 64, "vmcnt holds six bits");
+		__builtin_amdgcn_s_waitcnt(0x0070 | (OUT & 15) | (OUT >> 4) << 14); // vmcnt(OUT) lgkmcnt(0)
+		__syncthreads();
+	};
+	uint32_t issued = 0, fill = 0, use = 0;
+	auto next = [&] ()
+	{
+		if (++issued >= g.slabs) { ahead = 0; } // stays at the last slab
+		issue(fill);
+		fill = fill + 1 == SLABS ? 0 : fill + 1;
+	};
+	for (int k = 0; k < SLABS - 1; ++k) { next(); }
+	for (uint32_t s = 0; s < g.slabs;)
+	{
+		const uint32_t stop = CUT && s + FLUSH < g.slabs ? s + FLUSH : g.slabs;
+		for (; s < stop; ++s)
+		{
+			landed();
+			next();
+			multiply(use);
+			use = use + 1 == SLABS ? 0 : use + 1;
+		}
+		if constexpr (CUT)
+		{
+#pragma unroll
+			for (int i = 0; i < WT; ++i)
+			{
+#pragma unroll
+				for (int j = 0; j < WT; ++j)
+				{
+					sum[i][j] += acc[i][j];
+					acc[i][j] = f32x16{};
+				}
+			}
+		}
+	}
+	// nothing is on its way any more, LDS is free for the result
+	__builtin_amdgcn_s_waitcnt(0x0070);
+	__syncthreads();
+
+	const uint32_t i0 = bi * TILE + wi * (32 * WT), j0 = bj * TILE + wj * (32 * WT);
+	// the wave's tile as hi | lo << 16, [i][j]
+	uint32_t* meet = reinterpret_cast<uint32_t*>(lds) + wave * (32 * WT) * (32 * WT);
+#pragma unroll
+	for (int ti = 0; ti < WT; ++ti)
+	{
+#pragma unroll
+		for (int tj = 0; tj < WT; ++tj)
+		{
+			const f32x16 c = CUT ? sum[ti][tj] : acc[ti][tj];
+			const uint32_t j = j0 + tj * 32 + l32;
+#pragma unroll
+			for (int r = 0; r < 4; ++r)
+			{
+				// four neighbouring rows of column j
+				const uint32_t i = i0 + ti * 32 + 8 * r + 4 * half;
+				const uint64_t place = (uint64_t) (i / 32) * BLOCK + i % 32;
+				float v[4];
+#pragma unroll
+				for (int e = 0; e < 4; ++e) { v[e] = c[4 * r + e] * g.alpha; }
+				if constexpr (CUT)
+				{
+					const uint64_t where = batch * g.stride_add + (uint64_t) j * g.ldadd + i;
+					const float4 x = *reinterpret_cast<const float4*>(g.add32 + where);
+					v[0] += x.x * g.beta; v[1] += x.y * g.beta; v[2] += x.z * g.beta; v[3] += x.w * g.beta;
+					if constexpr (MODE == APPLY) { *reinterpret_cast<float4*>(g.out_t32 + where) = make_float4(v[0], v[1], v[2], v[3]); }
+				}
+				else if constexpr (MODE == FACTOR)
+				{
+					const f16* add = g.add + batch * g.stride_add + (uint64_t) j * g.ldadd + place;
+					const f16x4 hi = *reinterpret_cast<const f16x4*>(add), lo = *reinterpret_cast<const f16x4*>(add + 32);
+#pragma unroll
+					for (int e = 0; e < 4; ++e) { v[e] += ((float) hi[e] + (float) lo[e]) * g.beta; }
+				}
+				if constexpr (MODE == LAST)
+				{
+					float* last = g.last + batch * g.stride_l;
+					if (j < g.n)
+					{
+						if (g.tall)
+						{
+							float* p = last + (uint64_t) j * g.ldl + i;
+							if (i + 4 <= g.m) { *reinterpret_cast<f32x4_any*>(p) = f32x4_any{v[0], v[1], v[2], v[3]}; }
+							else
+							{
+#pragma unroll
+								for (int e = 0; e < 4; ++e) { if (i + e < g.m) { p[e] = v[e]; } }
+							}
+						}
+						else
+						{
+#pragma unroll
+							for (int e = 0; e < 4; ++e) { if (i + e < g.m) { last[(uint64_t) (i + e) * g.ldl + j] = v[e]; } }
+						}
+					}
+				}
+				else
+				{
+					f16x4 hi, lo;
+#pragma unroll
+					for (int e = 0; e < 4; ++e)
+					{
+						const Split s = split(v[e]);
+						hi[e] = s.hi;
+						lo[e] = s.lo;
+						meet[(ti * 32 + 8 * r + 4 * half + e) * (32 * WT) + tj * 32 + l32] =
+							(uint32_t) __builtin_bit_cast(uint16_t, s.hi) | (uint32_t) __builtin_bit_cast(uint16_t, s.lo) << 16;
+					}
+					f16* out = g.out_t + batch * g.stride_ot + (uint64_t) j * g.ldot + place;
+					*reinterpret_cast<f16x4*>(out) = hi;
+					*reinterpret_cast<f16x4*>(out + 32) = lo;
+				}
+			}
+		}
+	}
+	if constexpr (MODE != LAST)
+	{
+		// a tile on the diagonal of a symmetric result is complete
+		if (SYMMETRIC && bi == bj) { return; }
+		// the wave reads what it wrote itself
+		__builtin_amdgcn_s_waitcnt(0xc07f); // lgkmcnt(0)
+		__builtin_amdgcn_wave_barrier();
+		constexpr uint32_t QUADS = 8 * WT; // a row's groups of four
+#pragma unroll 4
+		for (uint32_t t = 0; t < 32 * WT * QUADS / TCG_WAVE; ++t)
+		{
+			const uint32_t e = t * TCG_WAVE + lane, i = e / QUADS, j = e % QUADS * 4;
+			const uint4 v = *reinterpret_cast<const uint4*>(meet + i * (32 * WT) + j);
+			uint2 hi, lo;
+			hi.x = (v.x & 0xffff) | v.y << 16; hi.y = (v.z & 0xffff) | v.w << 16;
+			lo.x = v.x >> 16 | (v.y & 0xffff0000u); lo.y = v.z >> 16 | (v.w & 0xffff0000u);
+			f16* out = g.out + batch * g.stride_o + (uint64_t) (i0 + i) * g.ldo + (uint64_t) ((j0 + j) / 32) * BLOCK + (j0 + j) % 32;
+			*reinterpret_cast<uint2*>(out) = hi;
+			*reinterpret_cast<uint2*>(out + 32) = lo;
+		}
+	}
+}
+
+// ---- double: elementwise parts between the products ------------------------------------
+
+__global__ __launch_bounds__(256) void ortho_scale_k (PrepArgs<double> a)
+{
+	__shared__ double red[4];
+	const double inv = inverse_norm(a, blockIdx.y, red);
+	const double* g = a.g + blockIdx.y * a.stride_g;
+	double* x = a.dense + blockIdx.y * a.stride_dense;
+	const uint64_t n = a.rows * a.cols;
+	for (uint64_t e = (uint64_t) blockIdx.x * 256 + threadIdx.x; e < n; e += (uint64_t) gridDim.x * 256)
+	{
+		// X dense: rows x cols, or transposed
+		const uint64_t row = a.tall ? e % a.rows : e / a.cols, col = a.tall ? e / a.rows : e % a.cols;
+		x[e] = g[row * a.ldg + col] * inv;
+	}
+}
+
+// out = alpha u + beta v over n elements a matrix
+__global__ __launch_bounds__(256) void ortho_join_k (uint64_t n, double alpha, const double* u, double beta, const double* v, double* out)
+{
+	for (uint64_t e = (uint64_t) blockIdx.x * 256 + threadIdx.x; e < n; e += (uint64_t) gridDim.x * 256)
+	{
+		out[e] = alpha * u[e] + beta * v[e];
+	}
+}
+
+// the dense X (transposed if `tall`) into the caller's rows x cols matrix
+__global__ __launch_bounds__(256) void ortho_store_k (PrepArgs<double> a, double* out, uint64_t ldo, uint64_t stride_o)
+{
+	const double* x = a.dense + blockIdx.y * a.stride_dense;
+	const uint64_t n = a.rows * a.cols;
+	for (uint64_t e = (uint64_t) blockIdx.x * 256 + threadIdx.x; e < n; e += (uint64_t) gridDim.x * 256)
+	{
+		const uint64_t row = e / a.cols, col = e % a.cols;
+		out[blockIdx.y * stride_o + row * ldo + col] = x[a.tall ? col * a.rows + row : e];
+	}
+}
+
+// ---- the host's side ---------------------------------------------------------------------
+
+struct Plan
+{
+	int steps;
+	double a, b, c;
+	// the largest singular value before step k, and the largest value of A and B in it
+	std::vector<double> x, gram, factor;
+};
+
+/// Follows the largest singular value any matrix can have: false where it grows out of bounds
+bool follow (Plan& p)
+{
+	if (!std::isfinite(p.a) || !std::isfinite(p.b) || !std::isfinite(p.c)) { return false; }
+	double top = 1.0001; // |X| <= 1, and the roundings of the norm
+	for (int k = 0; k <= p.steps; ++k)
+	{
+		if (!(top <= 1e6)) { return false; }
+		p.x.push_back(top);
+		double next = 0, factor = 0;
+		constexpr int POINTS = 2048;
+		for (int i = 0; i <= POINTS; ++i)
+		{
+			const double s = top * i / POINTS, q = s * s;
+			next = std::fmax(next, std::fabs(s * (p.a + q * (p.b + q * p.c))));
+			factor = std::fmax(factor, std::fabs(q * (p.b + q * p.c)));
+		}
+		p.gram.push_back(top * top);
+		p.factor.push_back(factor * 1.01);
+		// between two points the polynomial may rise a little higher
+		top = next * 1.01;
+		if (!(factor <= 1e12)) { return false; }
+	}
+	return true;
+}
+
+/// The power of two that puts `top` at 2^15, half of what a half can hold
+float scale_of (double top)
+{
+	if (!(top > 1e-9)) { top = 1e-9; }
+	int e;
+	(void) std::frexp(top, &e); // top < 2^e
+	return std::ldexp(1.f, 15 - e);
+}
+
+uint64_t padded (uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
+
+uint32_t norm_parts (uint64_t rows)
+{
+	const uint64_t want = (rows + 3) / 4;
+	return (uint32_t) (want < NORM_PARTS ? want : NORM_PARTS);
+}
+
+template <int WT, int SLABS, int MODE>
+hipError_t pair_launch (tcg_ctx* ctx, const PairArgs& g, uint64_t batch)
+{
+	constexpr int bytes = pair_lds<WT,SLABS>;
+	if constexpr (bytes > 65536)
+	{
+		// what a workgroup may hold beyond the 64 KiB that need no asking for
+		hipError_t err = hipFuncSetAttribute((const void*) ortho_pair_k<WT,SLABS,MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+		if (err != hipSuccess) { return err; }
+	}
+	ortho_pair_k<WT,SLABS,MODE><<<(unsigned) (g.tiles * batch), 256, bytes, ctx->stream>>>(g);
+	return hipGetLastError();
+}
+
+template <int WT, int SLABS>
+hipError_t pair_launch_mode (tcg_ctx* ctx, Product mode, const PairArgs& g, uint64_t batch)
+{
+	switch (mode)
+	{
+		case GRAM: return pair_launch<WT,SLABS,GRAM>(ctx, g, batch);
+		case FACTOR: return pair_launch<WT,SLABS,FACTOR>(ctx, g, batch);
+		case APPLY: return pair_launch<WT,SLABS,APPLY>(ctx, g, batch);
+		default: return pair_launch<WT,SLABS,LAST>(ctx, g, batch);
+	}
+}
+
+int ortho_float (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, uint64_t batch, const float* in, uint64_t ldg,
+	uint64_t stride_g, double eps, float* out, uint64_t ldo, uint64_t stride_o)
+{
+	const bool tall = rows > cols;
+	const uint64_t m = tall ? cols : rows, n = tall ? rows : cols;
+	// tiles of 128 x 128 where they fill the chip, of 64 x 64 elsewhere
+	const uint64_t big = padded(m, 128) / 128 * (padded(n, 128) / 128) * batch;
+	const int wt = big >= (uint64_t) ctx->num_cus ? 2 : 1;
+	const uint64_t tile = 64 * wt, mp = padded(m, tile), np = padded(n, tile);
+	const uint32_t tm = (uint32_t) (mp / tile), tn = (uint32_t) (np / tile);
+	TCG_REQUIRE(ctx, (uint64_t) tm * tn * batch < (1ull << 31), "tcg_orthogonalize: %llu matrices of %llu x %llu are too many",
+		(unsigned long long) batch, (unsigned long long) rows, (unsigned long long) cols);
+	// X, X^T and X^T in fp32 before and after a step, A, B; 32 bits an element each
+	const size_t xs = (size_t) mp * np * 2, as = (size_t) mp * mp * 2; // halves
+	const uint32_t parts = norm_parts(rows);
+	const size_t sums_bytes = ((size_t) batch * parts * sizeof(double) + 255) / 256 * 256;
+	const size_t bytes = sums_bytes + (6 * xs + 2 * as) * batch * sizeof(f16);
+	void* mem = nullptr;
+	int rc = tcg_alloc(ctx, bytes, &mem);
+	if (rc != TCG_OK) { return rc; }
+	f16* x[2], *xt[2];
+	float* xt32[2];
+	f16* p = reinterpret_cast<f16*>((char*) mem + sums_bytes);
+	for (int k = 0; k < 2; ++k)
+	{
+		x[k] = p; p += xs * batch;
+		xt[k] = p; p += xs * batch;
+		xt32[k] = reinterpret_cast<float*>(p); p += xs * batch;
+	}
+	f16* gram = p;
+	f16* factor = gram + as * batch;
+
+	PrepArgs<float> prep = {};
+	prep.g = in; prep.ldg = ldg; prep.stride_g = stride_g;
+	prep.rows = rows; prep.cols = cols;
+	prep.parts = parts; prep.sums = (double*) mem; prep.eps = eps;
+	prep.scale = scale_of(plan.x[0]);
+	prep.x = x[0]; prep.xt = xt[0]; prep.xt32 = xt32[0];
+	prep.ldx = np * 2; prep.ldxt = mp * 2;
+	prep.stride_x = prep.stride_xt = xs;
+	prep.tall = tall;
+	ortho_norm_k<float><<<dim3(parts, (unsigned) batch), 256, 0, ctx->stream>>>(prep);
+	const uint32_t tiles_x = (uint32_t) ((tall ? mp : np) / 64);
+	ortho_split_k<<<dim3((unsigned) (mp / 64 * (np / 64)), (unsigned) batch), 256, 0, ctx->stream>>>(prep, tiles_x);
+
+	hipError_t err = hipGetLastError();
+	auto launch = [&] (Product mode, const PairArgs& g)
+	{
+		if (err != hipSuccess) { return; }
+		err = wt == 2 ? pair_launch_mode<2,2>(ctx, mode, g, batch) : pair_launch_mode<1,4>(ctx, mode, g, batch);
+	};
+	for (int k = 0; k < plan.steps; ++k)
+	{
+		const int now = k & 1, next = now ^ 1;
+		const float sx = scale_of(plan.x[k]), sa = scale_of(plan.gram[k]), sb = scale_of(plan.factor[k]);
+		PairArgs g = {};
+		g.tiles_m = g.tiles_n = tm;
+		g.tiles = tm * (tm + 1) / 2;
+		g.p = g.q = x[now];
+		g.ldp = g.ldq = np * 2; g.stride_p = g.stride_q = xs;
+		g.slabs = (uint32_t) (np / 32);
+		g.alpha = sa / sx / sx;
+		g.out = g.out_t = gram;
+		g.ldo = g.ldot = mp * 2; g.stride_o = g.stride_ot = as;
+		launch(GRAM, g);
+		g.p = g.q = g.add = gram;
+		g.ldp = g.ldq = g.ldadd = mp * 2; g.stride_p = g.stride_q = g.stride_add = as;
+		g.slabs = (uint32_t) (mp / 32);
+		g.alpha = (float) plan.c * (sb / sa / sa);
+		g.beta = (float) plan.b * (sb / sa);
+		g.out = g.out_t = factor;
+		launch(FACTOR, g);
+		const bool last = k + 1 == plan.steps;
+		const float sn = last ? 1.f : scale_of(plan.x[k + 1]);
+		g.tiles_n = tn;
+		g.tiles = tm * tn;
+		g.p = factor;
+		g.q = xt[now];
+		g.ldq = mp * 2; g.stride_q = xs;
+		g.add32 = xt32[now]; g.out_t32 = xt32[next];
+		g.ldadd = mp; g.stride_add = xs / 2;
+		g.alpha = sn / sb / sx;
+		g.beta = (float) plan.a * (sn / sx);
+		g.out = x[next]; g.ldo = np * 2; g.stride_o = xs;
+		g.out_t = xt[next]; g.ldot = mp * 2; g.stride_ot = xs;
+		g.last = out; g.ldl = ldo; g.stride_l = stride_o;
+		g.m = (uint32_t) m; g.n = (uint32_t) n;
+		g.tall = tall;
+		launch(last ? LAST : APPLY, g);
+	}
+	rc = tcg_free(ctx, mem, bytes);
+	if (err != hipSuccess) { return tcg_fail(ctx, TCG_ERR_HIP, "launch of orthogonalize failed: %s", hipGetErrorString(err)); }
+	return rc;
+}
+
+int ortho_double (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, uint64_t batch, const double* in, uint64_t ldg,
+	uint64_t stride_g, double eps, double* out, uint64_t ldo, uint64_t stride_o)
+{
+	const bool tall = rows > cols;
+	const uint64_t m = tall ? cols : rows, n = tall ? rows : cols;
+	const uint32_t parts = norm_parts(rows);
+	const size_t sums_bytes = ((size_t) batch * parts * sizeof(double) + 255) / 256 * 256;
+	const size_t xs = (size_t) m * n, as = (size_t) m * m;
+	const size_t bytes = sums_bytes + (2 * xs + 2 * as) * batch * sizeof(double);
+	void* mem = nullptr;
+	int rc = tcg_alloc(ctx, bytes, &mem);
+	if (rc != TCG_OK) { return rc; }
+	double* x = (double*) ((char*) mem + sums_bytes);
+	double* y = x + xs * batch;
+	double* gram = y + xs * batch;
+	double* square = gram + as * batch;
+	PrepArgs<double> prep = {};
+	prep.g = in; prep.ldg = ldg; prep.stride_g = stride_g;
+	prep.rows = rows; prep.cols = cols;
+	prep.parts = parts; prep.sums = (double*) mem; prep.eps = eps;
+	prep.dense = x; prep.stride_dense = xs;
+	prep.tall = tall;
+	const unsigned sweep = tcg_grid(ctx, xs, 256, 8);
+	ortho_norm_k<double><<<dim3(parts, (unsigned) batch), 256, 0, ctx->stream>>>(prep);
+	ortho_scale_k<<<dim3(sweep, (unsigned) batch), 256, 0, ctx->stream>>>(prep);
+	for (int k = 0; k < plan.steps && rc == TCG_OK; ++k)
+	{
+		rc = tcg_gemm(ctx, TCG_DOUBLE, m, m, n, batch, x, n, xs, 0, x, n, xs, 1, gram, m, as);
+		if (rc != TCG_OK) { break; }
+		rc = tcg_gemm(ctx, TCG_DOUBLE, m, m, m, batch, gram, m, as, 0, gram, m, as, 0, square, m, as);
+		if (rc != TCG_OK) { break; }
+		ortho_join_k<<<tcg_grid(ctx, as * batch, 256, 8), 256, 0, ctx->stream>>>(as * batch, plan.b, gram, plan.c, square, square);
+		rc = tcg_gemm(ctx, TCG_DOUBLE, m, n, m, batch, square, m, as, 0, x, n, xs, 0, y, n, xs);
+		if (rc != TCG_OK) { break; }
+		ortho_join_k<<<tcg_grid(ctx, xs * batch, 256, 8), 256, 0, ctx->stream>>>(xs * batch, plan.a, x, 1., y, x);
+	}
+	if (rc == TCG_OK) { ortho_store_k<<<dim3(sweep, (unsigned) batch), 256, 0, ctx->stream>>>(prep, out, ldo, stride_o); }
+	hipError_t err = hipGetLastError();
+	const int freed = tcg_free(ctx, mem, bytes);
+	if (rc == TCG_OK) { rc = freed; }
+	if (rc == TCG_OK && err != hipSuccess) { return tcg_fail(ctx, TCG_ERR_HIP, "launch of orthogonalize failed: %s", hipGetErrorString(err)); }
+	return rc;
+}
+
+constexpr uint64_t MOST_ELEMENTS = 1ull << 33; // of one matrix, padding included; its temporaries take up to 32 bytes an element
+constexpr uint64_t MOST_BATCH = 65535;
+
+} // namespace
+
+extern "C" {
+
+int tcg_orthogonalize (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols, uint64_t batch, const void* in, uint64_t ldi,
+	uint64_t stride_i, int steps, const double coef[3], double eps, void* out, uint64_t ldo, uint64_t stride_o)
+{
+	if (!ctx) { return TCG_ERR_ARG; }
+	TCG_REQUIRE(ctx, dtype == TCG_FLOAT || dtype == TCG_DOUBLE, "tcg_orthogonalize: dtype %d is neither float nor double", dtype);
+	TCG_REQUIRE(ctx, ldi >= cols && ldo >= cols, "tcg_orthogonalize: leading dims %llu and %llu of rows of %llu elements",
+		(unsigned long long) ldi, (unsigned long long) ldo, (unsigned long long) cols);
+	TCG_REQUIRE(ctx, steps >= 1 && steps <= 64, "tcg_orthogonalize: %d steps: 1 to 64 are possible", steps);
+	TCG_REQUIRE(ctx, eps >= 0, "tcg_orthogonalize: eps %g is negative or not a number", eps);
+	TCG_REQUIRE(ctx, coef, "tcg_orthogonalize: NULL pointer");
+	if (0 == rows || 0 == cols || 0 == batch) { return TCG_OK; }
+	TCG_REQUIRE(ctx, in && out, "tcg_orthogonalize: NULL pointer");
+	TCG_REQUIRE(ctx, rows <= MOST_ELEMENTS / 128 && cols <= MOST_ELEMENTS / 128 && ldi <= MOST_ELEMENTS && ldo <= MOST_ELEMENTS &&
+		padded(rows, 128) <= MOST_ELEMENTS / padded(cols, 128) && batch <= MOST_BATCH,
+		"tcg_orthogonalize: %llu matrices of %llu x %llu are too many or too large",
+		(unsigned long long) batch, (unsigned long long) rows, (unsigned long long) cols);
+	// a matrix's rows end before the next matrix begins
+	const auto apart = [&] (uint64_t ld, uint64_t stride) { return batch == 1 || stride >= (rows - 1) * ld + cols; };
+	TCG_REQUIRE(ctx, apart(ldi, stride_i) && apart(ldo, stride_o), "tcg_orthogonalize: matrices %llu and %llu elements apart overlap",
+		(unsigned long long) stride_i, (unsigned long long) stride_o);
+	TCG_REQUIRE(ctx, in != out || (ldi == ldo && (batch == 1 || stride_i == stride_o)),
+		"tcg_orthogonalize: in place with another layout");
+	if (tcg_small_mode(ctx)) { TCG_SMALL_RETURN(ctx, tcg_small_unsupported(ctx, "an orthogonalised update")); }
+	tcg_device_scope device(ctx);
+	try
+	{
+		Plan plan;
+		plan.steps = steps;
+		plan.a = coef[0];
+		plan.b = coef[1];
+		plan.c = coef[2];
+		TCG_REQUIRE(ctx, follow(plan), "tcg_orthogonalize: with the polynomial %g s + %g s^3 + %g s^5 singular values grow past 1e6",
+			coef[0], coef[1], coef[2]);
+		if (batch == 1) { stride_i = stride_o = 0; }
+		return dtype == TCG_FLOAT ?
+			ortho_float(ctx, plan, rows, cols, batch, (const float*) in, ldi, stride_i, eps, (float*) out, ldo, stride_o) :
+			ortho_double(ctx, plan, rows, cols, batch, (const double*) in, ldi, stride_i, eps, (double*) out, ldo, stride_o);
+	}
+	catch (const std::bad_alloc&)
+	{
+		return tcg_fail(ctx, TCG_ERR_OOM, "tcg_orthogonalize: out of host memory");
+	}
+}
+
+} // extern "C"

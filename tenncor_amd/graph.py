@@ -553,6 +553,12 @@ class Api:
             out = self.add(out, self.extend_like(bias, out))
         return out
 
+    def orthogonalize(self, x, steps=5, epsilon=1e-7, coef=(3.4445, -4.7750, 2.0315)):
+        """The matrices over dims 0 and 1 of `x` with their singular values driven
+        towards one by `steps` of s -> coef[0] s + coef[1] s^3 + coef[2] s^5 from
+        x / (|x| + epsilon) on.  Has no derivative."""
+        return self.g.functor("ORTHOGONALIZE", [x], reals=[steps, epsilon, *coef])
+
     def cross_entropy(self, target, x):
         """loss.yml:40-59."""
         eps = float(np.finfo(np.float32).eps)
@@ -692,6 +698,24 @@ class Approx:
             update = a.assign(momentum, a.add(a.mul(discount_factor, momentum),
                                               a.mul(nodiscount, a.square(der))))
             out.append((x, a.assign_sub(x, a.div(a.mul(der, learning_rate), a.add(a.sqrt(update), self._epsilon(der, epsilon))))))
+        return out
+
+    def muon(self, error, variables, learning_rate=0.02, decay=0.95, nesterov=True, steps=5, epsilon=1e-7):
+        """For weight matrices: momentum = decay momentum + f'(x), and x moves along
+        the orthogonalised momentum (with `nesterov` along f'(x) + decay momentum):
+        x -= learning_rate sqrt(max(1, rows / columns)) orthogonalize(...).  Not one
+        of the reference's rules; variables that are no matrices are for the others."""
+        a = self.api
+        out = []
+        for x in variables:
+            if any(d != 1 for d in x.shape[2:]):
+                raise ValueError("muon updates matrices, not a variable of shape %s" % x.shape)
+        for x, der in zip(variables, self.g.derive(error, variables)):
+            momentum = self._variable_like(0, x, "momentum")
+            following = a.assign(momentum, a.add(a.mul(decay, momentum), der))
+            along = a.add(der, a.mul(decay, following)) if nesterov else following
+            rate = learning_rate * max(1.0, x.shape[1] / x.shape[0]) ** 0.5
+            out.append((x, a.assign_sub(x, a.mul(rate, a.orthogonalize(along, steps, epsilon)))))
         return out
 
     def apply_update(self, error, updates):

@@ -24,7 +24,7 @@ enum _GENERATED_OPCODE
 	ASSIGN_MUL, ASSIGN_DIV, CAST,
 	// nodes of this backend, behind those of cfg/ops.yml so that the codes of
 	// stored graphs stay what they are
-	LAYER_NORM, LAYER_NORM_DX, LAYER_NORM_DWEIGHT,
+	LAYER_NORM, LAYER_NORM_DX, LAYER_NORM_DWEIGHT, ORTHOGONALIZE,
 	_N_GENERATED_OPCODES
 };
 

@@ -631,6 +631,22 @@ EigenptrT layer_norm_dweight (teq::Shape outshape, const teq::TensptrsT& args, c
 	});
 }
 
+/// dims 0 and 1 are a matrix, the others count them
+template <typename T>
+EigenptrT orthogonalize (teq::Shape outshape, const teq::iTensor& in, const marsh::iAttributed& attrib)
+{
+	need_real<T>("orthogonalise");
+	OrthoParams params(attrib);
+	Shape8 shape = shape8(outshape);
+	uint64_t batch = 1;
+	for (size_t i = 2; i < shape.size(); ++i) { batch *= shape[i]; }
+	return make_op<T>(outshape, {&in}, [params, shape, batch](tcg_ctx* ctx, T* out, const std::vector<const void*>& args)
+	{
+		hip_check(tcg_orthogonalize(ctx, egen::device_type<T>(), shape[1], shape[0], batch, args[0], shape[0], shape[0] * shape[1],
+			params.steps, params.coef, params.epsilon, out, shape[0], shape[0] * shape[1]));
+	});
+}
+
 }
 
 namespace egen
@@ -705,6 +721,7 @@ void typed_exec (_GENERATED_OPCODE opcode, eigen::EigenptrT& out, teq::Shape out
 		case LAYER_NORM: out = eigen::layer_norm<T>(outshape, in, attrib); break;
 		case LAYER_NORM_DX: need(2); out = eigen::layer_norm_dx<T>(outshape, in, attrib); break;
 		case LAYER_NORM_DWEIGHT: need(2); out = eigen::layer_norm_dweight<T>(outshape, in, attrib); break;
+		case ORTHOGONALIZE: out = eigen::orthogonalize<T>(outshape, *in[0], attrib); break;
 		default: global::fatal("unknown opcode");
 	}
 }
@@ -728,7 +745,7 @@ void typed_exec (_GENERATED_OPCODE opcode, eigen::EigenptrT& out, teq::Shape out
 	TCH_OP_CASE(MACRO, CONCAT) TCH_OP_CASE(MACRO, ASSIGN) TCH_OP_CASE(MACRO, ASSIGN_ADD)\
 	TCH_OP_CASE(MACRO, ASSIGN_SUB) TCH_OP_CASE(MACRO, ASSIGN_MUL) TCH_OP_CASE(MACRO, ASSIGN_DIV)\
 	TCH_OP_CASE(MACRO, CAST) TCH_OP_CASE(MACRO, LAYER_NORM) TCH_OP_CASE(MACRO, LAYER_NORM_DX)\
-	TCH_OP_CASE(MACRO, LAYER_NORM_DWEIGHT) default: global::fatal("executing bad op"); }
+	TCH_OP_CASE(MACRO, LAYER_NORM_DWEIGHT) TCH_OP_CASE(MACRO, ORTHOGONALIZE) default: global::fatal("executing bad op"); }
 
 }
 

@@ -289,6 +289,29 @@ struct Packer<RealsT>
 	}
 };
 
+/// The attributes of ORTHOGONALIZE: `reals` = {steps, epsilon, and the
+/// coefficients of s, s^3 and s^5}
+struct OrthoParams final
+{
+	OrthoParams (const marsh::iAttributed& attrib)
+	{
+		RealsT reals;
+		Packer<RealsT>().unpack(reals, attrib);
+		if (reals.size() != 5) { global::throw_err("cannot ORTHOGONALIZE without steps, epsilon and three coefficients"); }
+		if (false == (reals[0] >= 1 && reals[0] <= 64) || reals[0] != (double) (int) reals[0])
+		{
+			global::throw_errf("cannot ORTHOGONALIZE in %g steps: 1 to 64 are possible", reals[0]);
+		}
+		if (false == (reals[1] >= 0)) { global::throw_errf("cannot ORTHOGONALIZE with epsilon %g", reals[1]); }
+		steps = (int) reals[0];
+		epsilon = reals[1];
+		for (int i = 0; i < 3; ++i) { coef[i] = reals[2 + i]; }
+	}
+
+	int steps;
+	double epsilon, coef[3];
+};
+
 inline void pack_attr (marsh::iAttributed&) {}
 
 template <typename T, typename ...ARGS>

@@ -426,7 +426,7 @@ const std::vector<Rule>& rule_table (void)
 		t[egen::LAYER_NORM] = rule_layer_norm;
 		for (auto code : {egen::RAND_UNIF, egen::EQ, egen::NEQ, egen::GT, egen::LT}) { t[code] = rule_zero; }
 		for (auto code : {egen::ASSIGN, egen::ASSIGN_ADD, egen::ASSIGN_SUB, egen::ASSIGN_MUL, egen::ASSIGN_DIV,
-			egen::ARGMAX, egen::LAYER_NORM_DX, egen::LAYER_NORM_DWEIGHT}) { t[code] = rule_refused; }
+			egen::ARGMAX, egen::LAYER_NORM_DX, egen::LAYER_NORM_DWEIGHT, egen::ORTHOGONALIZE}) { t[code] = rule_refused; }
 		return t;
 	}();
 	return table;

@@ -13,7 +13,7 @@ static const char* opnames[] = {
 	"STRIDE", "SCATTER", "POW", "ADD", "SUB", "MUL", "DIV", "MIN", "MAX", "EQ", "NEQ", "LT",
 	"GT", "MATMUL", "CONTRACT", "CONV", "SELECT", "CONCAT", "ASSIGN", "ASSIGN_ADD",
 	"ASSIGN_SUB", "ASSIGN_MUL", "ASSIGN_DIV", "CAST",
-	"LAYER_NORM", "LAYER_NORM_DX", "LAYER_NORM_DWEIGHT",
+	"LAYER_NORM", "LAYER_NORM_DX", "LAYER_NORM_DWEIGHT", "ORTHOGONALIZE",
 };
 
 std::string name_op (_GENERATED_OPCODE code)
@@ -375,6 +375,13 @@ teq::Shape parse_shape (_GENERATED_OPCODE opcode, const marsh::Maps& attrs, cons
 			(void) same_shape(opcode, {shapes[0], shapes[1]});
 			if (shapes.size() > 2) { need_norm_weight(opcode, shapes[1], rank, shapes[2]); }
 			return LAYER_NORM_DX == opcode ? shapes[1] : norm_weight_shape(shapes[1], rank);
+		}
+		case ORTHOGONALIZE: // matrices over dims 0 and 1, the other dims count them
+		{
+			if (shapes.size() != 1) { global::throw_errf("cannot %s %d arguments", name_op(opcode).c_str(), (int) shapes.size()); }
+			eigen::OrthoParams params(attrs);
+			(void) params;
+			return shapes.front();
 		}
 		case ASSIGN: case ASSIGN_ADD: case ASSIGN_SUB: case ASSIGN_MUL: case ASSIGN_DIV:
 		default:

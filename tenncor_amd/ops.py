@@ -150,6 +150,16 @@ def layer_norm_grad(up, x, weight=None, ndims=1, epsilon=1e-5, mean=None, rstd=N
     return dx, dweight, dbias
 
 
+def orthogonalize(x, steps=5, epsilon=1e-7, coef=(3.4445, -4.7750, 2.0315)):
+    """The matrices over dims 0 and 1 of `x`, each divided by its norm (plus epsilon),
+    after `steps` of s -> coef[0] s + coef[1] s^3 + coef[2] s^5 on its singular values."""
+    out = _new(x.ctx, x.shape, x)
+    cols, rows = x.shape[:2]
+    x.ctx.orthogonalize(x.dtype, rows, cols, capi.n_elems(x.shape[2:]), x.ptr, cols, rows * cols, out.ptr, cols, rows * cols,
+                        steps=steps, coef=coef, eps=epsilon)
+    return out
+
+
 def extend(x, bcast):
     """cfg/ops.yml:256-283."""
     b = capi.shape8(bcast)
