@@ -20,12 +20,11 @@
 //
 // What an error of X does is multiplied by up to a in each later step along the
 // weak directions of G, while one of A is read through B, which is small against
-// a there.  So a X is taken from X in fp32, and the sums of B X are cut every 256
-// indices and the parts added up apart: with both, results are as near to the
-// formulas as with fp32 products (1.6e-6 of the result's norm at 512 x 768; with
-// a X from the halves 3.2e-6, with uncut sums over 4096 indices 1e-5 and more).
+// a there.  So a X is taken from X in fp32, and the sums of B X are cut into parts
+// that are added up apart, so that neither a part nor their sum is a long chain of
+// roundings (sum_cut below).
 //
-// double: the same steps through the products of tcg_gemm.
+// double: the same steps on fp64 matrix instructions (78.6 TFLOP/s).
 #include "tcg_internal.hpp"
 
 #include <cmath>
@@ -42,7 +41,6 @@ typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 // A row of a split matrix: for every 32 elements 32 hi and then 32 lo, 128 bytes
 constexpr uint32_t BLOCK = 64; // halves
-constexpr uint32_t FLUSH = 8;  // slabs of 32 summed indices between two cuts of the sums of B X
 
 struct Split
 {
@@ -71,12 +69,12 @@ struct PrepArgs
 	double* sums; // [batch][parts]
 	double eps;
 	float scale;
-	// float: X and X^T as split matrices, mp x np padded; double: X dense
+	// float: X and X^T as split matrices, padded; double: dense, padded
 	f16* x;
 	f16* xt;
 	uint64_t ldx, stride_x, ldxt, stride_xt;
 	float* xt32; // X^T in fp32, rows of ldxt / 2
-	T* dense;
+	T* dense[2]; // X, X^T
 	uint64_t stride_dense;
 	bool tall; // X = G^T
 };
@@ -197,6 +195,7 @@ struct PairArgs
 	const f16* q;
 	uint64_t ldp, ldq, stride_p, stride_q;
 	uint32_t slabs; // of 32 summed indices
+	uint32_t cut;   // slabs between two cuts of the sums of B X
 	uint32_t tiles_m, tiles_n, tiles; // tiles: of one matrix (one triangle of them for GRAM and FACTOR)
 	// C alpha + add beta; row j of `add` holds what meets C(., j): the split matrix A
 	// (FACTOR), or X^T in fp32
@@ -215,6 +214,15 @@ struct PairArgs
 	uint32_t m, n;
 	bool tall;
 };
+
+/// Tile number `at` of a lower triangle, row after row
+__device__ __forceinline__ void triangle_place (uint32_t at, uint32_t& bi, uint32_t& bj)
+{
+	bi = (uint32_t) ((sqrtf(8.f * (float) at + 1.f) - 1.f) * 0.5f);
+	while (bi * (bi + 1) / 2 > at) { --bi; }
+	while ((bi + 1) * (bi + 2) / 2 <= at) { ++bi; }
+	bj = at - bi * (bi + 1) / 2;
+}
 
 /// Which 16 bytes of a row's 128 lie in which place in LDS: rows whose chunks a
 /// load of a matrix operand reads together never share banks
@@ -246,10 +254,7 @@ __global__ __launch_bounds__(256, 2) void ortho_pair_k (PairArgs g)
 	uint32_t bi, bj;
 	if constexpr (SYMMETRIC)
 	{
-		bi = (uint32_t) ((sqrtf(8.f * (float) tile + 1.f) - 1.f) * 0.5f);
-		while (bi * (bi + 1) / 2 > tile) { --bi; }
-		while ((bi + 1) * (bi + 2) / 2 <= tile) { ++bi; }
-		bj = tile - bi * (bi + 1) / 2;
+		triangle_place(tile, bi, bj);
 	}
 	else
 	{
@@ -345,7 +350,7 @@ __global__ __launch_bounds__(256, 2) void ortho_pair_k (PairArgs g)
 	for (int k = 0; k < SLABS - 1; ++k) { next(); }
 	for (uint32_t s = 0; s < g.slabs;)
 	{
-		const uint32_t stop = CUT && s + FLUSH < g.slabs ? s + FLUSH : g.slabs;
+		const uint32_t stop = CUT && s + g.cut < g.slabs ? s + g.cut : g.slabs;
 		for (; s < stop; ++s)
 		{
 			landed();
@@ -469,41 +474,413 @@ __global__ __launch_bounds__(256, 2) void ortho_pair_k (PairArgs g)
 	}
 }
 
-// ---- double: elementwise parts between the products ------------------------------------
+// ---- a small matrix in one workgroup ---------------------------------------------------
+// X in registers (fp32, 32 x 32 tiles dealt to the waves, up to two each), its halves
+// and those of A and B in LDS: all steps in one launch, bound by the barriers between
+// their parts instead of by fifteen launches (four matrices of 64 x 96: 76 us by
+// launches).  MT: tiles along m, at most 4; nt tiles along n.  The region of X holds
+// the halves of X (for A), the fp32 tiles of A and of A A on their way to being
+// split, and the halves of X^T (for B X), one after the other.
+constexpr int SMALL_STEPS = 64;
 
-__global__ __launch_bounds__(256) void ortho_scale_k (PrepArgs<double> a)
+struct SmallArgs
+{
+	const float* g;
+	uint64_t ldg, stride_g;
+	float* out;
+	uint64_t ldo, stride_o;
+	uint32_t m, n, nt;
+	uint32_t parts; // waves that share a tile of A, each a part of the summed index
+	int steps;
+	bool tall;
+	double eps;
+	float scale; // of X before the first step
+	// step k: A = gram C, B = factor C + keep A, X <- apply C + stay X
+	float gram[SMALL_STEPS], factor[SMALL_STEPS], keep[SMALL_STEPS], apply[SMALL_STEPS], stay[SMALL_STEPS];
+};
+
+/// LDS address of 16 bytes (8 indices of hi: chunk 0..3, of lo: 4..7) of row `row` in
+/// block `kb` of 32 summed indices of a matrix of `rows` rows
+__device__ __forceinline__ uint32_t small_place (uint32_t rows, uint32_t kb, uint32_t row, uint32_t chunk)
+{
+	return (kb * rows + row) * 128 + (chunk ^ swizzle(row)) * 16;
+}
+
+/// acc += P(rows of tile pi) Q(rows of tile qi)^T over blocks [from, to) of 32 indices
+__device__ __forceinline__ void small_product (f32x16& acc, const char* P, uint32_t p_rows, uint32_t pi, const char* Q, uint32_t q_rows, uint32_t qi,
+	uint32_t from, uint32_t to, uint32_t l32, uint32_t half)
+{
+	const uint32_t rp = pi * 32 + l32, rq = qi * 32 + l32;
+	for (uint32_t kb = from; kb < to; ++kb)
+	{
+#pragma unroll
+		for (uint32_t s = 0; s < 2; ++s)
+		{
+			const uint32_t c = 2 * s + half;
+			const f16x8 ph = *reinterpret_cast<const f16x8*>(P + small_place(p_rows, kb, rp, c));
+			const f16x8 pl = *reinterpret_cast<const f16x8*>(P + small_place(p_rows, kb, rp, c + 4));
+			const f16x8 qh = *reinterpret_cast<const f16x8*>(Q + small_place(q_rows, kb, rq, c));
+			const f16x8 ql = *reinterpret_cast<const f16x8*>(Q + small_place(q_rows, kb, rq, c + 4));
+			acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, acc, 0, 0, 0);
+			acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, acc, 0, 0, 0);
+			acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
+		}
+	}
+}
+
+__device__ __forceinline__ uint32_t packed (Split s)
+{
+	return (uint32_t) __builtin_bit_cast(uint16_t, s.hi) | (uint32_t) __builtin_bit_cast(uint16_t, s.lo) << 16;
+}
+
+template <int MT, int TILES>
+__global__ __launch_bounds__(1024) void ortho_small_k (SmallArgs g)
+{
+	extern __shared__ __attribute__((aligned(1024))) char lds[];
+	constexpr uint32_t ROWS = MT * 32;
+	const uint32_t cols = g.nt * 32;
+	char* X = lds;                                  // MT * nt tiles of 4 KiB
+	char* A = lds + MT * g.nt * 4096;               // MT * MT tiles
+	float* scratch = reinterpret_cast<float*>(lds); // tiles of fp32 in the region of X
+	const uint32_t waves = blockDim.x / TCG_WAVE, wave = threadIdx.x / TCG_WAVE, lane = threadIdx.x & (TCG_WAVE - 1);
+	const uint32_t l32 = lane & 31, half = lane >> 5;
+	const float* in = g.g + blockIdx.x * g.stride_g;
+	float* out = g.out + blockIdx.x * g.stride_o;
+
+	// the wave's tiles: element r of a lane is X(i, j), i = 32 ti + r % 4 + 8 (r / 4) + 4 half, j = 32 tj + l32
+	f32x16 x[TILES];
+	uint32_t ti[TILES], tj[TILES];
+	double sum = 0;
+#pragma unroll
+	for (int t = 0; t < TILES; ++t)
+	{
+		const uint32_t tile = wave + t * waves;
+		ti[t] = tile % MT;
+		tj[t] = tile / MT; // nt and more: no such tile
+		const uint32_t j = tj[t] * 32 + l32;
+#pragma unroll
+		for (int r = 0; r < 16; ++r)
+		{
+			const uint32_t i = ti[t] * 32 + r % 4 + 8 * (r / 4) + 4 * half;
+			float v = 0;
+			if (i < g.m && j < g.n) { v = g.tall ? in[(uint64_t) j * g.ldg + i] : in[(uint64_t) i * g.ldg + j]; }
+			x[t][r] = v;
+			sum += (double) v * v;
+		}
+	}
+	{
+		double* red = reinterpret_cast<double*>(lds);
+#pragma unroll
+		for (int d = TCG_WAVE / 2; d > 0; d >>= 1) { sum += __shfl_xor(sum, d); }
+		if (lane == 0) { red[wave] = sum; }
+		__syncthreads();
+		sum = 0;
+		for (uint32_t w = 0; w < waves; ++w) { sum += red[w]; }
+		__syncthreads();
+	}
+	const double inv = (double) g.scale / (::sqrt(sum) + g.eps);
+#pragma unroll
+	for (int t = 0; t < TILES; ++t)
+	{
+#pragma unroll
+		for (int r = 0; r < 16; ++r) { x[t][r] = (float) ((double) x[t][r] * inv); }
+	}
+
+	// fp32 tiles of MT x MT in `scratch`, `parts` of each to add up, into the halves at A;
+	// with KEEP the halves that are there count as well
+	auto settle = [&] (uint32_t parts, float alpha, float keep)
+	{
+		for (uint32_t e = threadIdx.x; e < MT * MT * 256; e += blockDim.x)
+		{
+			const uint32_t tile = e / 256, row = e % 256 / 8, col = e % 8 * 4;
+			const float* p = scratch + tile * 1024 + row * 32 + col;
+			float4 v = *reinterpret_cast<const float4*>(p);
+			for (uint32_t k = 1; k < parts; ++k)
+			{
+				const float4 u = *reinterpret_cast<const float4*>(p + k * (MT * MT * 1024));
+				v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+			}
+			const uint32_t i = tile % MT * 32 + row;
+			char* hi_at = A + small_place(ROWS, tile / MT, i, col / 8) + col % 8 * 2;
+			char* lo_at = A + small_place(ROWS, tile / MT, i, col / 8 + 4) + col % 8 * 2;
+			float w[4] = {v.x * alpha, v.y * alpha, v.z * alpha, v.w * alpha};
+			if (keep != 0)
+			{
+				const f16x4 hi = *reinterpret_cast<const f16x4*>(hi_at), lo = *reinterpret_cast<const f16x4*>(lo_at);
+#pragma unroll
+				for (int c = 0; c < 4; ++c) { w[c] += ((float) hi[c] + (float) lo[c]) * keep; }
+			}
+			f16x4 hi, lo;
+#pragma unroll
+			for (int c = 0; c < 4; ++c)
+			{
+				const Split s = split(w[c]);
+				hi[c] = s.hi;
+				lo[c] = s.lo;
+			}
+			*reinterpret_cast<f16x4*>(hi_at) = hi;
+			*reinterpret_cast<f16x4*>(lo_at) = lo;
+		}
+	};
+	auto put = [&] (const f32x16& c, uint32_t tile, uint32_t part)
+	{
+		float* p = scratch + (part * (MT * MT) + tile) * 1024 + l32;
+#pragma unroll
+		for (int r = 0; r < 16; ++r) { p[(r % 4 + 8 * (r / 4) + 4 * half) * 32] = c[r]; }
+	};
+
+	for (int k = 0; k < g.steps; ++k)
+	{
+		// the halves of X: rows i, summed index j.  Neighbouring lanes hold neighbouring j:
+		// an even lane takes both values of one row, the odd one those of the next
+#pragma unroll
+		for (int t = 0; t < TILES; ++t)
+		{
+			if (tj[t] >= g.nt) { continue; }
+			const bool odd = lane & 1;
+			const uint32_t j = l32 & ~1u;
+#pragma unroll
+			for (int r = 0; r < 16; r += 2)
+			{
+				const uint32_t first = packed(split(x[t][r])), second = packed(split(x[t][r + 1]));
+				const uint32_t got = __shfl_xor(odd ? first : second, 1);
+				const uint32_t left = odd ? got : first, right = odd ? second : got;
+				const uint32_t i = ti[t] * 32 + (r + (odd ? 1 : 0)) % 4 + 8 * (r / 4) + 4 * half;
+				*reinterpret_cast<uint32_t*>(X + small_place(ROWS, tj[t], i, j / 8) + j % 8 * 2) = (left & 0xffff) | right << 16;
+				*reinterpret_cast<uint32_t*>(X + small_place(ROWS, tj[t], i, j / 8 + 4) + j % 8 * 2) = left >> 16 | (right & 0xffff0000u);
+			}
+		}
+		__syncthreads();
+		// A = X X^T, `parts` waves a tile
+		f32x16 c = {};
+		const uint32_t tile = wave % (MT * MT), part = wave / (MT * MT);
+		if (part < g.parts)
+		{
+			small_product(c, X, ROWS, tile % MT, X, ROWS, tile / MT, g.nt * part / g.parts, g.nt * (part + 1) / g.parts, l32, half);
+		}
+		__syncthreads();
+		if (part < g.parts) { put(c, tile, part); }
+		__syncthreads();
+		settle(g.parts, g.gram[k], 0);
+		__syncthreads();
+		// B = b A + c A A (A is symmetric: its rows serve as both operands)
+		if (wave < MT * MT)
+		{
+			f32x16 d = {};
+			small_product(d, A, ROWS, tile % MT, A, ROWS, tile / MT, 0, MT, l32, half);
+			put(d, tile, 0);
+		}
+		__syncthreads();
+		settle(1, g.factor[k], g.keep[k]);
+		__syncthreads();
+		// the halves of X^T: rows j, summed index i; a lane holds four neighbouring i
+#pragma unroll
+		for (int t = 0; t < TILES; ++t)
+		{
+			if (tj[t] >= g.nt) { continue; }
+			const uint32_t j = tj[t] * 32 + l32;
+#pragma unroll
+			for (int r = 0; r < 4; ++r)
+			{
+				const uint32_t i = 8 * r + 4 * half;
+				f16x4 hi, lo;
+#pragma unroll
+				for (int e = 0; e < 4; ++e)
+				{
+					const Split s = split(x[t][4 * r + e]);
+					hi[e] = s.hi;
+					lo[e] = s.lo;
+				}
+				*reinterpret_cast<f16x4*>(X + small_place(cols, ti[t], j, i / 8) + i % 8 * 2) = hi;
+				*reinterpret_cast<f16x4*>(X + small_place(cols, ti[t], j, i / 8 + 4) + i % 8 * 2) = lo;
+			}
+		}
+		__syncthreads();
+		// X <- a X + B X
+#pragma unroll
+		for (int t = 0; t < TILES; ++t)
+		{
+			if (tj[t] >= g.nt) { continue; }
+			f32x16 d = {};
+			small_product(d, A, ROWS, ti[t], X, cols, tj[t], 0, MT, l32, half);
+#pragma unroll
+			for (int r = 0; r < 16; ++r) { x[t][r] = x[t][r] * g.stay[k] + d[r] * g.apply[k]; }
+		}
+		__syncthreads();
+	}
+#pragma unroll
+	for (int t = 0; t < TILES; ++t)
+	{
+		const uint32_t j = tj[t] * 32 + l32;
+#pragma unroll
+		for (int r = 0; r < 16; ++r)
+		{
+			const uint32_t i = ti[t] * 32 + r % 4 + 8 * (r / 4) + 4 * half;
+			if (i < g.m && j < g.n)
+			{
+				if (g.tall) { out[(uint64_t) j * g.ldo + i] = x[t][r]; }
+				else { out[(uint64_t) i * g.ldo + j] = x[t][r]; }
+			}
+		}
+	}
+}
+
+// ---- double -----------------------------------------------------------------------------
+// The same steps over dense doubles, padded with zeros to multiples of 64 rows and
+// columns, both operands with the summed index along memory.  A wave holds a 32 x 32
+// tile (v_mfma_f64_16x16x4: lane i + 16 q supplies element (i, q) of an operand and
+// holds elements (4 r + q, i) of the result) and reads its operands straight from
+// memory, 16 bytes a lane: the matrix instructions take 32 cycles each, eight of
+// them for four loads, so the loads of the next indices are out long before they
+// are used and nothing has to be staged.  KSPLIT = 4: the four waves of a workgroup
+// share one tile, every fourth group of eight summed indices each, and their parts
+// are added in wave order (few tiles); KSPLIT = 1: a wave to each quarter of a 64 x 64
+// tile (the operands are read half as often).
+
+typedef double f64x2 __attribute__((ext_vector_type(2)));
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+struct DoubleArgs
+{
+	// C(i, j) = sum_k p(i, k) q(j, k)
+	const double* p;
+	const double* q;
+	uint64_t ldp, ldq, stride_p, stride_q;
+	uint32_t depth; // summed indices, a multiple of 64
+	uint32_t tiles_m, tiles_n, tiles;
+	const double* add; // C alpha + add beta
+	uint64_t ldadd, stride_add;
+	double alpha, beta;
+	double* out;   // (i, j)
+	double* out_t; // (j, i)
+	uint64_t ldo, ldot, stride_o, stride_ot;
+	double* last;
+	uint64_t ldl, stride_l;
+	uint32_t m, n;
+	bool tall;
+};
+
+template <int KSPLIT, int MODE>
+__global__ __launch_bounds__(256) void ortho_double_k (DoubleArgs g)
+{
+	constexpr bool SYMMETRIC = MODE == GRAM || MODE == FACTOR;
+	constexpr uint32_t TILE = KSPLIT == 1 ? 64 : 32;
+	constexpr uint32_t PITCH = TILE + 1;
+	__shared__ double meet[KSPLIT * TILE * PITCH];
+	const uint32_t total = gridDim.x, xcd = blockIdx.x % 8, each = total / 8, more = total % 8;
+	const uint32_t at = xcd * each + (xcd < more ? xcd : more) + blockIdx.x / 8;
+	const uint32_t batch = at / g.tiles, tile = at % g.tiles;
+	uint32_t bi, bj;
+	if constexpr (SYMMETRIC) { triangle_place(tile, bi, bj); }
+	else
+	{
+		bi = tile % g.tiles_m;
+		bj = tile / g.tiles_m;
+	}
+	const uint32_t wave = threadIdx.x / TCG_WAVE, lane = threadIdx.x & (TCG_WAVE - 1);
+	const uint32_t l16 = lane & 15, quarter = lane >> 4;
+	const uint32_t wi = KSPLIT == 1 ? wave / 2 : 0, wj = KSPLIT == 1 ? wave % 2 : 0;
+	const double* p = g.p + batch * g.stride_p + (uint64_t) (bi * TILE + wi * 32 + l16) * g.ldp + 2 * quarter;
+	const double* q = g.q + batch * g.stride_q + (uint64_t) (bj * TILE + wj * 32 + l16) * g.ldq + 2 * quarter;
+	f64x4 acc[2][2] = {};
+	constexpr uint32_t STEP = KSPLIT == 1 ? 8 : 32; // between a wave's groups of eight indices
+	constexpr uint32_t AHEAD = 2;                   // groups loaded together
+	for (uint32_t k = KSPLIT == 1 ? 0 : wave * 8; k < g.depth; k += STEP * AHEAD)
+	{
+		f64x2 a[AHEAD][2], b[AHEAD][2];
+#pragma unroll
+		for (uint32_t h = 0; h < AHEAD; ++h)
+		{
+#pragma unroll
+			for (int t = 0; t < 2; ++t)
+			{
+				a[h][t] = *reinterpret_cast<const f64x2*>(p + (uint64_t) t * 16 * g.ldp + k + h * STEP);
+				b[h][t] = *reinterpret_cast<const f64x2*>(q + (uint64_t) t * 16 * g.ldq + k + h * STEP);
+			}
+		}
+#pragma unroll
+		for (uint32_t h = 0; h < AHEAD; ++h)
+		{
+#pragma unroll
+			for (int e = 0; e < 2; ++e)
+			{
+#pragma unroll
+				for (int i = 0; i < 2; ++i)
+				{
+#pragma unroll
+					for (int j = 0; j < 2; ++j)
+					{
+						acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64(a[h][i][e], b[h][j][e], acc[i][j], 0, 0, 0);
+					}
+				}
+			}
+		}
+	}
+	double* mine = meet + (KSPLIT == 1 ? 0 : wave * TILE * PITCH);
+#pragma unroll
+	for (int i = 0; i < 2; ++i)
+	{
+#pragma unroll
+		for (int j = 0; j < 2; ++j)
+		{
+#pragma unroll
+			for (int r = 0; r < 4; ++r)
+			{
+				mine[(wi * 32 + i * 16 + 4 * r + quarter) * PITCH + wj * 32 + j * 16 + l16] = acc[i][j][r];
+			}
+		}
+	}
+	__syncthreads();
+	const uint32_t i0 = bi * TILE, j0 = bj * TILE;
+	// the result where its rows run along memory; what is kept transposed goes by LDS
+	for (uint32_t e = threadIdx.x; e < TILE * TILE; e += 256)
+	{
+		const uint32_t i = e / TILE, j = e % TILE;
+		double v = 0;
+#pragma unroll
+		for (int w = 0; w < KSPLIT; ++w) { v += meet[w * TILE * PITCH + i * PITCH + j]; }
+		v *= g.alpha;
+		if constexpr (MODE != GRAM) { v += g.beta * g.add[batch * g.stride_add + (uint64_t) (i0 + i) * g.ldadd + j0 + j]; }
+		if constexpr (MODE != LAST) { g.out[batch * g.stride_o + (uint64_t) (i0 + i) * g.ldo + j0 + j] = v; }
+		else if (!g.tall && i0 + i < g.m && j0 + j < g.n) { g.last[batch * g.stride_l + (uint64_t) (i0 + i) * g.ldl + j0 + j] = v; }
+		meet[i * PITCH + j] = v; // read by this lane alone until now
+	}
+	__syncthreads();
+	if ((SYMMETRIC && bi == bj) || (MODE == LAST && !g.tall)) { return; }
+	for (uint32_t e = threadIdx.x; e < TILE * TILE; e += 256)
+	{
+		const uint32_t j = e / TILE, i = e % TILE;
+		const double v = meet[i * PITCH + j];
+		if constexpr (MODE != LAST) { g.out_t[batch * g.stride_ot + (uint64_t) (j0 + j) * g.ldot + i0 + i] = v; }
+		else if (i0 + i < g.m && j0 + j < g.n) { g.last[batch * g.stride_l + (uint64_t) (j0 + j) * g.ldl + i0 + i] = v; }
+	}
+}
+
+// X = G / (|G| + eps) and X^T, padded: a 64 x 64 tile a workgroup
+__global__ __launch_bounds__(256) void ortho_scale_k (PrepArgs<double> a, uint32_t tiles_x)
 {
 	__shared__ double red[4];
-	const double inv = inverse_norm(a, blockIdx.y, red);
-	const double* g = a.g + blockIdx.y * a.stride_g;
-	double* x = a.dense + blockIdx.y * a.stride_dense;
-	const uint64_t n = a.rows * a.cols;
-	for (uint64_t e = (uint64_t) blockIdx.x * 256 + threadIdx.x; e < n; e += (uint64_t) gridDim.x * 256)
+	__shared__ double tile[64][65];
+	const uint32_t batch = blockIdx.y;
+	const double inv = inverse_norm(a, batch, red);
+	const uint64_t r0 = (uint64_t) (blockIdx.x / tiles_x) * 64, c0 = (uint64_t) (blockIdx.x % tiles_x) * 64;
+	const double* g = a.g + batch * a.stride_g;
+	double* along = a.dense[a.tall] + batch * a.stride_dense;
+	double* across = a.dense[!a.tall] + batch * a.stride_dense;
+	const uint64_t ld_along = a.tall ? a.ldxt : a.ldx, ld_across = a.tall ? a.ldx : a.ldxt;
+	for (uint32_t e = threadIdx.x; e < 64 * 64; e += 256)
 	{
-		// X dense: rows x cols, or transposed
-		const uint64_t row = a.tall ? e % a.rows : e / a.cols, col = a.tall ? e / a.rows : e % a.cols;
-		x[e] = g[row * a.ldg + col] * inv;
+		const uint32_t r = e / 64, c = e % 64;
+		double v = 0;
+		if (r0 + r < a.rows && c0 + c < a.cols) { v = g[(r0 + r) * a.ldg + c0 + c] * inv; }
+		tile[r][c] = v;
+		along[(r0 + r) * ld_along + c0 + c] = v;
 	}
-}
-
-// out = alpha u + beta v over n elements a matrix
-__global__ __launch_bounds__(256) void ortho_join_k (uint64_t n, double alpha, const double* u, double beta, const double* v, double* out)
-{
-	for (uint64_t e = (uint64_t) blockIdx.x * 256 + threadIdx.x; e < n; e += (uint64_t) gridDim.x * 256)
+	__syncthreads();
+	for (uint32_t e = threadIdx.x; e < 64 * 64; e += 256)
 	{
-		out[e] = alpha * u[e] + beta * v[e];
-	}
-}
-
-// the dense X (transposed if `tall`) into the caller's rows x cols matrix
-__global__ __launch_bounds__(256) void ortho_store_k (PrepArgs<double> a, double* out, uint64_t ldo, uint64_t stride_o)
-{
-	const double* x = a.dense + blockIdx.y * a.stride_dense;
-	const uint64_t n = a.rows * a.cols;
-	for (uint64_t e = (uint64_t) blockIdx.x * 256 + threadIdx.x; e < n; e += (uint64_t) gridDim.x * 256)
-	{
-		const uint64_t row = e / a.cols, col = e % a.cols;
-		out[blockIdx.y * stride_o + row * ldo + col] = x[a.tall ? col * a.rows + row : e];
+		const uint32_t c = e / 64, r = e % 64;
+		across[(c0 + c) * ld_across + r0 + r] = tile[r][c];
 	}
 }
 
@@ -552,6 +929,16 @@ float scale_of (double top)
 	return std::ldexp(1.f, 15 - e);
 }
 
+/// A slab is six additions to a sum; cut so that a part and the sum of the parts are
+/// chains of about one length.  Distance from the formulas at 768 rows (24 slabs):
+/// cut every 2 slabs 2.9e-6, every 8 3.6e-6; at 4096 (128 slabs): every 2 4.3e-6,
+/// every 8 3.1e-6; fp32 products that are never cut 1.3e-5 and 2.9e-5
+uint32_t sum_cut (uint32_t slabs)
+{
+	const uint32_t cut = (uint32_t) std::lround(std::sqrt(slabs / 6.));
+	return cut < 2 ? 2 : cut;
+}
+
 uint64_t padded (uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
 uint32_t norm_parts (uint64_t rows)
@@ -586,11 +973,79 @@ hipError_t pair_launch_mode (tcg_ctx* ctx, Product mode, const PairArgs& g, uint
 	}
 }
 
+/// Tiles of LDS a matrix takes in ortho_small_k, 0: it is not one of its
+int small_tiles (uint64_t m, uint64_t n)
+{
+	const uint64_t mt = (m + 31) / 32, nt = (n + 31) / 32;
+	if (mt > 4 || nt > 32 || mt * nt > 32) { return 0; }
+	const int tiles = (int) (mt * nt + mt * mt);
+	return tiles <= 39 ? tiles : 0; // 156 of 160 KiB
+}
+
+template <int MT>
+hipError_t small_launch (tcg_ctx* ctx, const SmallArgs& g, uint64_t batch, int lds_tiles)
+{
+	const unsigned tiles = MT * g.nt, waves = tiles < 16 ? tiles : 16, bytes = lds_tiles * 4096;
+	const void* kernel = tiles > 16 ? (const void*) ortho_small_k<MT,2> : (const void*) ortho_small_k<MT,1>;
+	if (bytes > 65536)
+	{
+		hipError_t err = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int) bytes);
+		if (err != hipSuccess) { return err; }
+	}
+	if (tiles > 16) { ortho_small_k<MT,2><<<(unsigned) batch, waves * TCG_WAVE, bytes, ctx->stream>>>(g); }
+	else { ortho_small_k<MT,1><<<(unsigned) batch, waves * TCG_WAVE, bytes, ctx->stream>>>(g); }
+	return hipGetLastError();
+}
+
+int ortho_small (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, uint64_t batch, const float* in, uint64_t ldg,
+	uint64_t stride_g, double eps, float* out, uint64_t ldo, uint64_t stride_o, int lds_tiles)
+{
+	SmallArgs g = {};
+	g.g = in; g.ldg = ldg; g.stride_g = stride_g;
+	g.out = out; g.ldo = ldo; g.stride_o = stride_o;
+	g.tall = rows > cols;
+	g.m = (uint32_t) (g.tall ? cols : rows);
+	g.n = (uint32_t) (g.tall ? rows : cols);
+	const uint32_t mt = (g.m + 31) / 32;
+	g.nt = (g.n + 31) / 32;
+	const uint32_t waves = mt * g.nt < 16 ? mt * g.nt : 16;
+	// the parts' tiles have to fit where X lies
+	g.parts = waves / (mt * mt);
+	if (g.parts > g.nt / mt) { g.parts = g.nt / mt; }
+	g.steps = plan.steps;
+	g.eps = eps;
+	g.scale = scale_of(plan.x[0]);
+	for (int k = 0; k < plan.steps; ++k)
+	{
+		const float sx = scale_of(plan.x[k]), sa = scale_of(plan.gram[k]), sb = scale_of(plan.factor[k]);
+		const float sn = k + 1 == plan.steps ? 1.f : scale_of(plan.x[k + 1]);
+		g.gram[k] = sa / sx / sx;
+		g.factor[k] = (float) plan.c * (sb / sa / sa);
+		g.keep[k] = (float) plan.b * (sb / sa);
+		g.apply[k] = sn / sb / sx;
+		g.stay[k] = (float) plan.a * (sn / sx);
+	}
+	hipError_t err;
+	switch (mt)
+	{
+		case 1: err = small_launch<1>(ctx, g, batch, lds_tiles); break;
+		case 2: err = small_launch<2>(ctx, g, batch, lds_tiles); break;
+		case 3: err = small_launch<3>(ctx, g, batch, lds_tiles); break;
+		default: err = small_launch<4>(ctx, g, batch, lds_tiles); break;
+	}
+	if (err != hipSuccess) { return tcg_fail(ctx, TCG_ERR_HIP, "launch of orthogonalize failed: %s", hipGetErrorString(err)); }
+	return TCG_OK;
+}
+
 int ortho_float (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, uint64_t batch, const float* in, uint64_t ldg,
 	uint64_t stride_g, double eps, float* out, uint64_t ldo, uint64_t stride_o)
 {
 	const bool tall = rows > cols;
 	const uint64_t m = tall ? cols : rows, n = tall ? rows : cols;
+	if (const int tiles = small_tiles(m, n))
+	{
+		return ortho_small(ctx, plan, rows, cols, batch, in, ldg, stride_g, eps, out, ldo, stride_o, tiles);
+	}
 	// tiles of 128 x 128 where they fill the chip, of 64 x 64 elsewhere
 	const uint64_t big = padded(m, 128) / 128 * (padded(n, 128) / 128) * batch;
 	const int wt = big >= (uint64_t) ctx->num_cus ? 2 : 1;
@@ -667,6 +1122,7 @@ int ortho_float (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, u
 		g.ldq = mp * 2; g.stride_q = xs;
 		g.add32 = xt32[now]; g.out_t32 = xt32[next];
 		g.ldadd = mp; g.stride_add = xs / 2;
+		g.cut = sum_cut(g.slabs);
 		g.alpha = sn / sb / sx;
 		g.beta = (float) plan.a * (sn / sx);
 		g.out = x[next]; g.ldo = np * 2; g.stride_o = xs;
@@ -681,47 +1137,96 @@ int ortho_float (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, u
 	return rc;
 }
 
+template <int KSPLIT>
+void double_launch (tcg_ctx* ctx, Product mode, const DoubleArgs& g, uint64_t batch)
+{
+	const unsigned grid = (unsigned) (g.tiles * batch);
+	switch (mode)
+	{
+		case GRAM: ortho_double_k<KSPLIT,GRAM><<<grid, 256, 0, ctx->stream>>>(g); break;
+		case FACTOR: ortho_double_k<KSPLIT,FACTOR><<<grid, 256, 0, ctx->stream>>>(g); break;
+		case APPLY: ortho_double_k<KSPLIT,APPLY><<<grid, 256, 0, ctx->stream>>>(g); break;
+		default: ortho_double_k<KSPLIT,LAST><<<grid, 256, 0, ctx->stream>>>(g); break;
+	}
+}
+
 int ortho_double (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, uint64_t batch, const double* in, uint64_t ldg,
 	uint64_t stride_g, double eps, double* out, uint64_t ldo, uint64_t stride_o)
 {
 	const bool tall = rows > cols;
 	const uint64_t m = tall ? cols : rows, n = tall ? rows : cols;
+	const uint64_t mp = padded(m, 64), np = padded(n, 64);
+	const size_t xs = (size_t) mp * np, as = (size_t) mp * mp;
 	const uint32_t parts = norm_parts(rows);
 	const size_t sums_bytes = ((size_t) batch * parts * sizeof(double) + 255) / 256 * 256;
-	const size_t xs = (size_t) m * n, as = (size_t) m * m;
-	const size_t bytes = sums_bytes + (2 * xs + 2 * as) * batch * sizeof(double);
+	const size_t bytes = sums_bytes + (4 * xs + 2 * as) * batch * sizeof(double);
+	TCG_REQUIRE(ctx, mp / 32 * (np / 32) * batch < (1ull << 31), "tcg_orthogonalize: %llu matrices of %llu x %llu are too many",
+		(unsigned long long) batch, (unsigned long long) rows, (unsigned long long) cols);
 	void* mem = nullptr;
 	int rc = tcg_alloc(ctx, bytes, &mem);
 	if (rc != TCG_OK) { return rc; }
-	double* x = (double*) ((char*) mem + sums_bytes);
-	double* y = x + xs * batch;
-	double* gram = y + xs * batch;
-	double* square = gram + as * batch;
+	double* x[2][2]; // [before, after a step][X, X^T]
+	double* at = (double*) ((char*) mem + sums_bytes);
+	for (int k = 0; k < 4; ++k, at += xs * batch) { x[k / 2][k % 2] = at; }
+	double* gram = at;
+	double* factor = gram + as * batch;
 	PrepArgs<double> prep = {};
 	prep.g = in; prep.ldg = ldg; prep.stride_g = stride_g;
 	prep.rows = rows; prep.cols = cols;
 	prep.parts = parts; prep.sums = (double*) mem; prep.eps = eps;
-	prep.dense = x; prep.stride_dense = xs;
+	prep.dense[0] = x[0][0]; prep.dense[1] = x[0][1];
+	prep.stride_dense = xs;
+	prep.ldx = np; prep.ldxt = mp;
 	prep.tall = tall;
-	const unsigned sweep = tcg_grid(ctx, xs, 256, 8);
 	ortho_norm_k<double><<<dim3(parts, (unsigned) batch), 256, 0, ctx->stream>>>(prep);
-	ortho_scale_k<<<dim3(sweep, (unsigned) batch), 256, 0, ctx->stream>>>(prep);
-	for (int k = 0; k < plan.steps && rc == TCG_OK; ++k)
+	ortho_scale_k<<<dim3((unsigned) (mp / 64 * (np / 64)), (unsigned) batch), 256, 0, ctx->stream>>>(prep, (uint32_t) ((tall ? mp : np) / 64));
+	auto launch = [&] (Product mode, DoubleArgs& g, uint64_t height, uint64_t width)
 	{
-		rc = tcg_gemm(ctx, TCG_DOUBLE, m, m, n, batch, x, n, xs, 0, x, n, xs, 1, gram, m, as);
-		if (rc != TCG_OK) { break; }
-		rc = tcg_gemm(ctx, TCG_DOUBLE, m, m, m, batch, gram, m, as, 0, gram, m, as, 0, square, m, as);
-		if (rc != TCG_OK) { break; }
-		ortho_join_k<<<tcg_grid(ctx, as * batch, 256, 8), 256, 0, ctx->stream>>>(as * batch, plan.b, gram, plan.c, square, square);
-		rc = tcg_gemm(ctx, TCG_DOUBLE, m, n, m, batch, square, m, as, 0, x, n, xs, 0, y, n, xs);
-		if (rc != TCG_OK) { break; }
-		ortho_join_k<<<tcg_grid(ctx, xs * batch, 256, 8), 256, 0, ctx->stream>>>(xs * batch, plan.a, x, 1., y, x);
+		// 64 x 64 tiles where they fill the chip twice, else the summed index shared by the waves of a tile
+		const bool wide = height / 64 * (width / 64) * batch >= 2 * (uint64_t) ctx->num_cus;
+		const uint32_t tile = wide ? 64 : 32;
+		g.tiles_m = (uint32_t) (height / tile);
+		g.tiles_n = (uint32_t) (width / tile);
+		g.tiles = mode == GRAM || mode == FACTOR ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
+		if (wide) { double_launch<1>(ctx, mode, g, batch); }
+		else { double_launch<4>(ctx, mode, g, batch); }
+	};
+	for (int k = 0; k < plan.steps; ++k)
+	{
+		double** now = x[k & 1];
+		double** next = x[(k & 1) ^ 1];
+		DoubleArgs g = {};
+		g.p = g.q = now[0];
+		g.ldp = g.ldq = np; g.stride_p = g.stride_q = xs;
+		g.depth = (uint32_t) np;
+		g.alpha = 1;
+		g.out = g.out_t = gram;
+		g.ldo = g.ldot = mp; g.stride_o = g.stride_ot = as;
+		launch(GRAM, g, mp, mp);
+		g.p = g.q = g.add = gram;
+		g.ldp = g.ldq = g.ldadd = mp; g.stride_p = g.stride_q = g.stride_add = as;
+		g.depth = (uint32_t) mp;
+		g.alpha = plan.c;
+		g.beta = plan.b;
+		g.out = g.out_t = factor;
+		launch(FACTOR, g, mp, mp);
+		g.p = factor;
+		g.q = now[1];
+		g.ldq = mp; g.stride_q = xs;
+		g.add = now[0];
+		g.ldadd = np; g.stride_add = xs;
+		g.alpha = 1;
+		g.beta = plan.a;
+		g.out = next[0]; g.ldo = np; g.stride_o = xs;
+		g.out_t = next[1]; g.ldot = mp; g.stride_ot = xs;
+		g.last = out; g.ldl = ldo; g.stride_l = stride_o;
+		g.m = (uint32_t) m; g.n = (uint32_t) n;
+		g.tall = tall;
+		launch(k + 1 == plan.steps ? LAST : APPLY, g, mp, np);
 	}
-	if (rc == TCG_OK) { ortho_store_k<<<dim3(sweep, (unsigned) batch), 256, 0, ctx->stream>>>(prep, out, ldo, stride_o); }
 	hipError_t err = hipGetLastError();
-	const int freed = tcg_free(ctx, mem, bytes);
-	if (rc == TCG_OK) { rc = freed; }
-	if (rc == TCG_OK && err != hipSuccess) { return tcg_fail(ctx, TCG_ERR_HIP, "launch of orthogonalize failed: %s", hipGetErrorString(err)); }
+	rc = tcg_free(ctx, mem, bytes);
+	if (err != hipSuccess) { return tcg_fail(ctx, TCG_ERR_HIP, "launch of orthogonalize failed: %s", hipGetErrorString(err)); }
 	return rc;
 }
 
