@@ -479,8 +479,8 @@ __global__ __launch_bounds__(256, 2) void ortho_pair_k (PairArgs g)
 // and those of A and B in LDS: all steps in one launch, bound by the barriers between
 // their parts instead of by fifteen launches (four matrices of 64 x 96: 76 us by
 // launches).  MT: tiles along m, at most 4; nt tiles along n.  The region of X holds
-// the halves of X (for A), the fp32 tiles of A and of A A on their way to being
-// split, and the halves of X^T (for B X), one after the other.
+// the halves of X (for A), where waves share a tile of A their fp32 parts of it, and
+// the halves of X^T (for B X), one after the other.
 constexpr int SMALL_STEPS = 64;
 
 struct SmallArgs
@@ -511,6 +511,7 @@ __device__ __forceinline__ void small_product (f32x16& acc, const char* P, uint3
 	uint32_t from, uint32_t to, uint32_t l32, uint32_t half)
 {
 	const uint32_t rp = pi * 32 + l32, rq = qi * 32 + l32;
+#pragma unroll 1
 	for (uint32_t kb = from; kb < to; ++kb)
 	{
 #pragma unroll
@@ -548,7 +549,9 @@ __global__ __launch_bounds__(1024) void ortho_small_k (SmallArgs g)
 	float* out = g.out + blockIdx.x * g.stride_o;
 
 	// the wave's tiles: element r of a lane is X(i, j), i = 32 ti + r % 4 + 8 (r / 4) + 4 half, j = 32 tj + l32
-	f32x16 x[TILES];
+	// (single values, not the vectors of the matrix instructions: those are moved whole when
+	// registers run short)
+	float x[TILES][16];
 	uint32_t ti[TILES], tj[TILES];
 	double sum = 0;
 #pragma unroll
@@ -586,51 +589,35 @@ __global__ __launch_bounds__(1024) void ortho_small_k (SmallArgs g)
 		for (int r = 0; r < 16; ++r) { x[t][r] = (float) ((double) x[t][r] * inv); }
 	}
 
-	// fp32 tiles of MT x MT in `scratch`, `parts` of each to add up, into the halves at A;
-	// with KEEP the halves that are there count as well
-	auto settle = [&] (uint32_t parts, float alpha, float keep)
-	{
-		for (uint32_t e = threadIdx.x; e < MT * MT * 256; e += blockDim.x)
-		{
-			const uint32_t tile = e / 256, row = e % 256 / 8, col = e % 8 * 4;
-			const float* p = scratch + tile * 1024 + row * 32 + col;
-			float4 v = *reinterpret_cast<const float4*>(p);
-			for (uint32_t k = 1; k < parts; ++k)
-			{
-				const float4 u = *reinterpret_cast<const float4*>(p + k * (MT * MT * 1024));
-				v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
-			}
-			const uint32_t i = tile % MT * 32 + row;
-			char* hi_at = A + small_place(ROWS, tile / MT, i, col / 8) + col % 8 * 2;
-			char* lo_at = A + small_place(ROWS, tile / MT, i, col / 8 + 4) + col % 8 * 2;
-			float w[4] = {v.x * alpha, v.y * alpha, v.z * alpha, v.w * alpha};
-			if (keep != 0)
-			{
-				const f16x4 hi = *reinterpret_cast<const f16x4*>(hi_at), lo = *reinterpret_cast<const f16x4*>(lo_at);
-#pragma unroll
-				for (int c = 0; c < 4; ++c) { w[c] += ((float) hi[c] + (float) lo[c]) * keep; }
-			}
-			f16x4 hi, lo;
-#pragma unroll
-			for (int c = 0; c < 4; ++c)
-			{
-				const Split s = split(w[c]);
-				hi[c] = s.hi;
-				lo[c] = s.lo;
-			}
-			*reinterpret_cast<f16x4*>(hi_at) = hi;
-			*reinterpret_cast<f16x4*>(lo_at) = lo;
-		}
-	};
-	auto put = [&] (const f32x16& c, uint32_t tile, uint32_t part)
-	{
-		float* p = scratch + (part * (MT * MT) + tile) * 1024 + l32;
-#pragma unroll
-		for (int r = 0; r < 16; ++r) { p[(r % 4 + 8 * (r / 4) + 4 * half) * 32] = c[r]; }
-	};
-
+	const uint32_t own_lane = lane;
 	for (int k = 0; k < g.steps; ++k)
 	{
+		// a value the compiler cannot follow from step to step: it would otherwise work out
+		// every LDS address before the first step and spill them (2100 registers of them)
+		uint32_t lane = own_lane;
+		asm volatile("" : "+v"(lane));
+		const uint32_t l32 = lane & 31, half = lane >> 5;
+		// a tile of a matrix of `rows` rows, where it lies transposed: a lane holds four
+		// neighbouring summed indices of row 32 t + l32
+		auto put_across = [l32, half] (char* where, uint32_t rows, uint32_t kb, uint32_t t, auto value)
+		{
+#pragma unroll
+			for (int r = 0; r < 4; ++r)
+			{
+				const uint32_t i = 8 * r + 4 * half;
+				f16x4 hi, lo;
+#pragma unroll
+				for (int e = 0; e < 4; ++e)
+				{
+					const Split s = split(value(4 * r + e));
+					hi[e] = s.hi;
+					lo[e] = s.lo;
+				}
+				*reinterpret_cast<f16x4*>(where + small_place(rows, kb, t * 32 + l32, i / 8) + i % 8 * 2) = hi;
+				*reinterpret_cast<f16x4*>(where + small_place(rows, kb, t * 32 + l32, i / 8 + 4) + i % 8 * 2) = lo;
+				__builtin_amdgcn_sched_barrier(0); // one group after the other: 128 registers a lane are few
+			}
+		};
 		// the halves of X: rows i, summed index j.  Neighbouring lanes hold neighbouring j:
 		// an even lane takes both values of one row, the odd one those of the next
 #pragma unroll
@@ -648,52 +635,63 @@ __global__ __launch_bounds__(1024) void ortho_small_k (SmallArgs g)
 				const uint32_t i = ti[t] * 32 + (r + (odd ? 1 : 0)) % 4 + 8 * (r / 4) + 4 * half;
 				*reinterpret_cast<uint32_t*>(X + small_place(ROWS, tj[t], i, j / 8) + j % 8 * 2) = (left & 0xffff) | right << 16;
 				*reinterpret_cast<uint32_t*>(X + small_place(ROWS, tj[t], i, j / 8 + 4) + j % 8 * 2) = left >> 16 | (right & 0xffff0000u);
+				__builtin_amdgcn_sched_barrier(0);
 			}
 		}
 		__syncthreads();
-		// A = X X^T, `parts` waves a tile
-		f32x16 c = {};
-		const uint32_t tile = wave % (MT * MT), part = wave / (MT * MT);
+		// A = X X^T: tile (ai, aj) in the wave that keeps it, with `parts` waves a tile.  A and B
+		// are symmetric: what a wave holds of one goes where it lies transposed, and rows of A
+		// serve as both operands of A A
+		f32x16 a = {};
+		const uint32_t tile = wave % (MT * MT), part = wave / (MT * MT), ai = tile % MT, aj = tile / MT;
 		if (part < g.parts)
 		{
-			small_product(c, X, ROWS, tile % MT, X, ROWS, tile / MT, g.nt * part / g.parts, g.nt * (part + 1) / g.parts, l32, half);
+			small_product(a, X, ROWS, ai, X, ROWS, aj, g.nt * part / g.parts, g.nt * (part + 1) / g.parts, l32, half);
 		}
-		__syncthreads();
-		if (part < g.parts) { put(c, tile, part); }
-		__syncthreads();
-		settle(g.parts, g.gram[k], 0);
-		__syncthreads();
-		// B = b A + c A A (A is symmetric: its rows serve as both operands)
-		if (wave < MT * MT)
+		if (g.parts > 1)
 		{
-			f32x16 d = {};
-			small_product(d, A, ROWS, tile % MT, A, ROWS, tile / MT, 0, MT, l32, half);
-			put(d, tile, 0);
+			// the other waves' parts by way of the region of X, added in their order
+			__syncthreads();
+			if (part > 0 && part < g.parts)
+			{
+				float* p = scratch + ((part - 1) * (MT * MT) + tile) * 1024 + l32;
+#pragma unroll
+				for (int r = 0; r < 16; ++r) { p[(r % 4 + 8 * (r / 4) + 4 * half) * 32] = a[r]; }
+			}
+			__syncthreads();
+			if (part == 0)
+			{
+#pragma unroll 1
+				for (uint32_t w = 1; w < g.parts; ++w)
+				{
+					const float* p = scratch + ((w - 1) * (MT * MT) + tile) * 1024 + l32;
+#pragma unroll
+					for (int r = 0; r < 16; ++r) { a[r] += p[(r % 4 + 8 * (r / 4) + 4 * half) * 32]; }
+				}
+			}
+		}
+		float kept[16] = {};
+		if (part == 0)
+		{
+			const float gram = g.gram[k];
+#pragma unroll
+			for (int r = 0; r < 16; ++r) { kept[r] = a[r] * gram; }
+			put_across(A, ROWS, ai, aj, [&kept] (int r) { return kept[r]; });
 		}
 		__syncthreads();
-		settle(1, g.factor[k], g.keep[k]);
+		f32x16 b = {};
+		if (part == 0) { small_product(b, A, ROWS, ai, A, ROWS, aj, 0, MT, l32, half); }
 		__syncthreads();
-		// the halves of X^T: rows j, summed index i; a lane holds four neighbouring i
+		if (part == 0)
+		{
+			// A itself from the registers
+			const float factor = g.factor[k], keep = g.keep[k];
+			put_across(A, ROWS, ai, aj, [&kept, &b, factor, keep] (int r) { return kept[r] * keep + b[r] * factor; });
+		}
 #pragma unroll
 		for (int t = 0; t < TILES; ++t)
 		{
-			if (tj[t] >= g.nt) { continue; }
-			const uint32_t j = tj[t] * 32 + l32;
-#pragma unroll
-			for (int r = 0; r < 4; ++r)
-			{
-				const uint32_t i = 8 * r + 4 * half;
-				f16x4 hi, lo;
-#pragma unroll
-				for (int e = 0; e < 4; ++e)
-				{
-					const Split s = split(x[t][4 * r + e]);
-					hi[e] = s.hi;
-					lo[e] = s.lo;
-				}
-				*reinterpret_cast<f16x4*>(X + small_place(cols, ti[t], j, i / 8) + i % 8 * 2) = hi;
-				*reinterpret_cast<f16x4*>(X + small_place(cols, ti[t], j, i / 8 + 4) + i % 8 * 2) = lo;
-			}
+			if (tj[t] < g.nt) { put_across(X, cols, ti[t], tj[t], [&x, t] (int r) { return x[t][r]; }); }
 		}
 		__syncthreads();
 		// X <- a X + B X
@@ -703,8 +701,9 @@ __global__ __launch_bounds__(1024) void ortho_small_k (SmallArgs g)
 			if (tj[t] >= g.nt) { continue; }
 			f32x16 d = {};
 			small_product(d, A, ROWS, ti[t], X, cols, tj[t], 0, MT, l32, half);
+			const float stay = g.stay[k], apply = g.apply[k];
 #pragma unroll
-			for (int r = 0; r < 16; ++r) { x[t][r] = x[t][r] * g.stay[k] + d[r] * g.apply[k]; }
+			for (int r = 0; r < 16; ++r) { x[t][r] = x[t][r] * stay + d[r] * apply; }
 		}
 		__syncthreads();
 	}
@@ -901,21 +900,30 @@ bool follow (Plan& p)
 	double top = 1.0001; // |X| <= 1, and the roundings of the norm
 	for (int k = 0; k <= p.steps; ++k)
 	{
-		if (!(top <= 1e6)) { return false; }
+		if (!(top <= 1e6)) { return false; } // a NaN as well
 		p.x.push_back(top);
+		// both are largest at an end or where their slope is zero: with q = s^2,
+		// p' = a + 3 b q + 5 c q^2 and (b q + c q^2)' = b + 2 c q
 		double next = 0, factor = 0;
-		constexpr int POINTS = 2048;
-		for (int i = 0; i <= POINTS; ++i)
+		auto at = [&] (double q)
 		{
-			const double s = top * i / POINTS, q = s * s;
-			next = std::fmax(next, std::fabs(s * (p.a + q * (p.b + q * p.c))));
+			if (!(q > 0 && q <= top * top)) { return; }
+			next = std::fmax(next, std::sqrt(q) * std::fabs(p.a + q * (p.b + q * p.c)));
 			factor = std::fmax(factor, std::fabs(q * (p.b + q * p.c)));
+		};
+		at(top * top);
+		if (p.c != 0) { at(-p.b / (2 * p.c)); }
+		const double inner = 9 * p.b * p.b - 20 * p.a * p.c;
+		if (p.c != 0 && inner >= 0)
+		{
+			at((-3 * p.b + std::sqrt(inner)) / (10 * p.c));
+			at((-3 * p.b - std::sqrt(inner)) / (10 * p.c));
 		}
+		else if (p.c == 0 && p.b != 0) { at(-p.a / (3 * p.b)); }
+		if (!(next <= 1e300 && factor <= 1e12)) { return false; }
 		p.gram.push_back(top * top);
-		p.factor.push_back(factor * 1.01);
-		// between two points the polynomial may rise a little higher
-		top = next * 1.01;
-		if (!(factor <= 1e12)) { return false; }
+		p.factor.push_back(factor * 1.0001);
+		top = next * 1.0001;
 	}
 	return true;
 }
@@ -1009,9 +1017,10 @@ int ortho_small (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, u
 	const uint32_t mt = (g.m + 31) / 32;
 	g.nt = (g.n + 31) / 32;
 	const uint32_t waves = mt * g.nt < 16 ? mt * g.nt : 16;
-	// the parts' tiles have to fit where X lies
+	// the parts' tiles have to fit where X lies; more than four cost more to add up than they save
 	g.parts = waves / (mt * mt);
 	if (g.parts > g.nt / mt) { g.parts = g.nt / mt; }
+	if (g.parts > 4) { g.parts = 4; }
 	g.steps = plan.steps;
 	g.eps = eps;
 	g.scale = scale_of(plan.x[0]);
