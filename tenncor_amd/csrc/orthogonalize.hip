@@ -55,6 +55,12 @@ __device__ __forceinline__ Split split (float v)
 	return s;
 }
 
+/// hi | lo << 16
+__device__ __forceinline__ uint32_t packed (Split s)
+{
+	return (uint32_t) __builtin_bit_cast(uint16_t, s.hi) | (uint32_t) __builtin_bit_cast(uint16_t, s.lo) << 16;
+}
+
 // ---- the norm, and the first split -------------------------------------------------
 
 constexpr uint32_t NORM_PARTS = 256; // workgroups that sum one matrix at most
@@ -73,7 +79,7 @@ struct PrepArgs
 	f16* x;
 	f16* xt;
 	uint64_t ldx, stride_x, ldxt, stride_xt;
-	float* xt32; // X^T in fp32, rows of ldxt / 2
+	float* x32; // X in fp32, place32
 	T* dense[2]; // X, X^T
 	uint64_t stride_dense;
 	bool tall; // X = G^T
@@ -123,6 +129,13 @@ __device__ __forceinline__ double inverse_norm (const PrepArgs<T>& a, uint32_t b
 	return 1. / (::sqrt(group_sum(sum, red)) + a.eps);
 }
 
+/// Where the 32 x 32 block (bi, bj) of a matrix of `rows` rows keeps its values in fp32:
+/// lane l's four values (8 r + 4 (l / 32) + 0..3, l % 32) at 256 r + 4 l
+__device__ __forceinline__ uint64_t place32 (uint32_t rows, uint32_t bi, uint32_t bj)
+{
+	return ((uint64_t) bj * (rows / 32) + bi) * 1024;
+}
+
 // X = G / (|G| + eps) and X^T as split matrices, a 64 x 64 tile a workgroup; what
 // lies outside G is zero
 __global__ __launch_bounds__(256) void ortho_split_k (PrepArgs<float> a, uint32_t tiles_x)
@@ -162,19 +175,12 @@ __global__ __launch_bounds__(256) void ortho_split_k (PrepArgs<float> a, uint32_
 		f16* q = across + (c0 + r) * ld_across + (r0 + c) / 32 * BLOCK + c % 32;
 		*reinterpret_cast<f16x4*>(q) = thi;
 		*reinterpret_cast<f16x4*>(q + 32) = tlo;
-		float4 wide;
-		uint64_t row, col;
-		if (a.tall)
-		{
-			wide = make_float4(tile[r][c], tile[r][c + 1], tile[r][c + 2], tile[r][c + 3]);
-			row = r0 + r; col = c0 + c;
-		}
-		else
-		{
-			wide = make_float4(tile[c][r], tile[c + 1][r], tile[c + 2][r], tile[c + 3][r]);
-			row = c0 + r; col = r0 + c;
-		}
-		*reinterpret_cast<float4*>(a.xt32 + batch * (a.stride_xt / 2) + row * (a.ldxt / 2) + col) = wide;
+		// X(i, j) in fp32: four neighbouring i, which are G's columns if it is tall
+		const float4 wide = a.tall ? make_float4(tile[r][c], tile[r][c + 1], tile[r][c + 2], tile[r][c + 3]) :
+			make_float4(tile[c][r], tile[c + 1][r], tile[c + 2][r], tile[c + 3][r]);
+		const uint32_t row = (uint32_t) (a.tall ? c0 : r0) + c, col = (uint32_t) (a.tall ? r0 : c0) + r;
+		float* to = a.x32 + batch * (a.stride_x / 2) + place32((uint32_t) (a.ldxt / 2), row / 32, col / 32);
+		*reinterpret_cast<float4*>(to + row % 32 / 8 * 256 + (row % 8 / 4 * 32 + col % 32) * 4) = wide;
 	}
 }
 
@@ -194,19 +200,19 @@ struct PairArgs
 	const f16* p;
 	const f16* q;
 	uint64_t ldp, ldq, stride_p, stride_q;
+	uint32_t rows_p, rows_q; // padded to whole blocks of 32
 	uint32_t slabs; // of 32 summed indices
 	uint32_t cut;   // slabs between two cuts of the sums of B X
 	uint32_t tiles_m, tiles_n, tiles; // tiles: of one matrix (one triangle of them for GRAM and FACTOR)
-	// C alpha + add beta; row j of `add` holds what meets C(., j): the split matrix A
-	// (FACTOR), or X^T in fp32
-	const f16* add;
-	const float* add32;
-	uint64_t ldadd, stride_add; // in elements of the one that is given
+	// C alpha + add beta, and that in fp32 as it is in the registers of the matrix
+	// instructions (`place32`): nothing but the next product of the same tiles reads it
+	const float* add32;  // NULL for GRAM
+	float* out32;        // NULL for FACTOR and LAST
+	uint64_t stride32;
 	float alpha, beta;
 	// the result: row i, and row j of its transposed
 	f16* out;
 	f16* out_t;
-	float* out_t32; // APPLY: X^T in fp32, laid out like add32
 	uint64_t ldo, ldot, stride_o, stride_ot;
 	// LAST
 	float* last;
@@ -228,21 +234,19 @@ __device__ __forceinline__ void triangle_place (uint32_t at, uint32_t& bi, uint3
 /// load of a matrix operand reads together never share banks
 __device__ __forceinline__ uint32_t swizzle (uint32_t row) { return ((row >> 1) & 7) ^ ((row & 1) << 2); }
 
-// WT: 32 x 32 blocks along each side of a wave's tile; four waves 2 x 2.  SLABS of
-// 32 summed indices have room in LDS: one is multiplied while SLABS - 1 are on
-// their way.
+// WT: 32 x 32 blocks along each side of a wave's tile; four waves 2 x 2 make a tile of
+// the result.  SLABS slabs of 32 summed indices have room in LDS.
 template <int WT, int SLABS>
-constexpr int pair_lds = SLABS * 2 * 64 * WT * 128;
+constexpr int pair_lds = SLABS * 2 * 64 * WT * 128 > 16 * 32 * WT * (32 * WT + 1) ? SLABS * 2 * 64 * WT * 128 : 16 * 32 * WT * (32 * WT + 1);
 
 template <int WT, int SLABS, int MODE>
-__global__ __launch_bounds__(256, 2) void ortho_pair_k (PairArgs g)
+__global__ __launch_bounds__(256) void ortho_pair_k (PairArgs g)
 {
 	constexpr int TILE = 64 * WT;
 	constexpr int OPERAND = TILE * 128; // bytes of an operand's slab in LDS
 	constexpr int LOADS = 2 * WT;       // a wave's loads per operand and slab
 	constexpr bool SYMMETRIC = MODE == GRAM || MODE == FACTOR;
 	constexpr bool CUT = MODE == APPLY || MODE == LAST;
-	static_assert(pair_lds<WT,SLABS> >= 4 * 4 * (32 * WT) * (32 * WT), "the result's way through LDS");
 	extern __shared__ __attribute__((aligned(1024))) char lds[];
 
 	// consecutive workgroups go to the XCDs in turn: each XCD gets a run of
@@ -272,91 +276,119 @@ __global__ __launch_bounds__(256, 2) void ortho_pair_k (PairArgs g)
 	{
 		const uint32_t r = wave * (16 * WT) + i * 8 + lane / 8;
 		const uint32_t chunk = (lane & 7) ^ swizzle(r);
-		from[0][i] = g.p + batch * g.stride_p + ((uint64_t) bi * TILE + r) * g.ldp + chunk * 8;
-		from[1][i] = g.q + batch * g.stride_q + ((uint64_t) bj * TILE + r) * g.ldq + chunk * 8;
+		// rows past the end: the last one again, never stored
+		const uint32_t rp = bi * TILE + r, rq = bj * TILE + r;
+		from[0][i] = g.p + batch * g.stride_p + (uint64_t) (rp < g.rows_p ? rp : g.rows_p - 1) * g.ldp + chunk * 8;
+		from[1][i] = g.q + batch * g.stride_q + (uint64_t) (rq < g.rows_q ? rq : g.rows_q - 1) * g.ldq + chunk * 8;
 		const uint32_t base = (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) char*) lds + (wave * (16 * WT) + i * 8) * 128;
 		to[0][i] = __builtin_amdgcn_readfirstlane(base);
 		to[1][i] = __builtin_amdgcn_readfirstlane(base + OPERAND);
 	}
 	uint32_t ahead = BLOCK;
-	// the next slab of both operands into LDS buffer `b`, 16 bytes a lane straight from memory.
-	// The instruction itself: for its builtin the compiler waits for every such load
-	// before any later read of LDS.  The s_nop is the wait state between the write of M0
-	// and its use.
-	auto issue = [&] (uint32_t b)
+	// load number `l` of a wave's 2 LOADS of a slab into LDS buffer `b`, 16 bytes a lane
+	// straight from memory.  The instruction itself: for its builtin the compiler waits for
+	// every such load before any later read of LDS.  The s_nop is the wait state between
+	// the write of M0 and its use.
+	auto issue = [&] (uint32_t b, int l)
 	{
-#pragma unroll
-		for (int o = 0; o < 2; ++o)
-		{
-#pragma unroll
-			for (int i = 0; i < LOADS; ++i)
-			{
-				asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-					: : "v"(from[o][i]), "s"(to[o][i] + b * 2 * OPERAND) : "memory", "m0");
-				from[o][i] += ahead;
-			}
-		}
+		const int o = l / LOADS, i = l % LOADS;
+		asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+			: : "v"(from[o][i]), "s"(to[o][i] + b * 2 * OPERAND) : "memory", "m0");
+		from[o][i] += ahead;
 	};
 	f32x16 acc[WT][WT] = {}, sum[WT][WT] = {};
-	auto multiply = [&] (uint32_t b)
+	// what a lane supplies to the matrix instructions of half a slab (16 summed indices):
+	// hi and lo of its WT rows of P, then of Q
+	struct Half
 	{
-		const char* P = lds + b * 2 * OPERAND;
-		const char* Q = P + OPERAND;
+		f16x8 v[4][WT];
+	};
+	constexpr int READS = 4 * WT, PRODUCTS = 3 * WT * WT;
+	auto read = [&] (Half& h, uint32_t b, uint32_t s, int n)
+	{
+		const int t = n / 4, what = n % 4, o = what / 2;
+		const uint32_t row = (o ? wj : wi) * (32 * WT) + t * 32 + l32;
+		const uint32_t chunk = (2 * s + half + 4 * (what % 2)) ^ swizzle(row);
+		h.v[what][t] = *reinterpret_cast<const f16x8*>(lds + (b * 2 + o) * OPERAND + row * 128 + chunk * 16);
+	};
+	// The matrix instructions of half a slab (lo and hi, hi and lo, hi and hi: neighbours
+	// never wait for each other's sums) and, after number m of them, what goes out
+	// meanwhile: `also(m)`.  A wave's instructions are issued in order, and an LDS read
+	// or a load holds the ones behind it up for as long as the waves share that unit:
+	// all of them together in front of the products left the matrix unit idle half of
+	// the time (1530 instead of 770 cycles a slab at WT = 2).
+	auto multiply = [&] (const Half& h, auto also)
+	{
 #pragma unroll
-		for (int s = 0; s < 2; ++s)
+		for (int kind = 0; kind < 3; ++kind)
 		{
-			f16x8 ph[WT], pl[WT], qh[WT], ql[WT];
-#pragma unroll
-			for (int t = 0; t < WT; ++t)
-			{
-				const uint32_t rp = wi * (32 * WT) + t * 32 + l32, rq = wj * (32 * WT) + t * 32 + l32;
-				const uint32_t c = 2 * s + half, fp = swizzle(rp), fq = swizzle(rq);
-				ph[t] = *reinterpret_cast<const f16x8*>(P + rp * 128 + (c ^ fp) * 16);
-				pl[t] = *reinterpret_cast<const f16x8*>(P + rp * 128 + ((c + 4) ^ fp) * 16);
-				qh[t] = *reinterpret_cast<const f16x8*>(Q + rq * 128 + (c ^ fq) * 16);
-				ql[t] = *reinterpret_cast<const f16x8*>(Q + rq * 128 + ((c + 4) ^ fq) * 16);
-			}
 #pragma unroll
 			for (int i = 0; i < WT; ++i)
 			{
 #pragma unroll
 				for (int j = 0; j < WT; ++j)
 				{
-					acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
-					acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
-					acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
+					acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(h.v[kind == 0 ? 1 : 0][i], h.v[kind == 1 ? 3 : 2][j], acc[i][j], 0, 0, 0);
+					also((kind * WT + i) * WT + j);
+					__builtin_amdgcn_sched_barrier(0);
 				}
 			}
 		}
 	};
-	// Every step issues the loads of one slab (past the end none is left: the last
-	// one again, never used), so with the loads of SLABS - 2 slabs out the slab
-	// of the step has landed: loads complete in order.  Behind the barrier every wave
-	// is done with the buffer that the step's loads overwrite.
+	// Half a slab is multiplied while the next half is on its way out of LDS.  Between the
+	// halves of slab s: slab s + 1 has landed (loads complete in order, and those of
+	// SLABS - 3 later slabs may still be out), and behind the barrier every wave is done
+	// with slab s - 1, whose buffer the loads of slab s + SLABS - 1 overwrite (past the
+	// end none is left: the last one again, never used).
 	auto landed = [] ()
 	{
-		constexpr int OUT = (SLABS - 2) * 2 * LOADS;
-		static_assert(OUT < 64, "vmcnt holds six bits");
-		__builtin_amdgcn_s_waitcnt(0x0070 | (OUT & 15) | (OUT >> 4) << 14); // vmcnt(OUT) lgkmcnt(0)
-		__syncthreads();
+		constexpr int OUT = (SLABS - 3) * 2 * LOADS;
+		static_assert(OUT >= 0 && OUT < 64, "vmcnt holds six bits");
+		__builtin_amdgcn_sched_barrier(0);
+		__builtin_amdgcn_s_waitcnt(0x0f70 | (OUT & 15) | (OUT >> 4) << 14); // vmcnt(OUT)
+		__builtin_amdgcn_s_barrier();
+		__builtin_amdgcn_sched_barrier(0);
 	};
+	const uint32_t slabs = g.slabs;
 	uint32_t issued = 0, fill = 0, use = 0;
-	auto next = [&] ()
+	auto begin = [&] () { if (++issued >= slabs) { ahead = 0; } }; // stays at the last slab
+	auto done = [&] () { fill = fill + 1 == SLABS ? 0 : fill + 1; };
+	auto whole = [&] ()
 	{
-		if (++issued >= g.slabs) { ahead = 0; } // stays at the last slab
-		issue(fill);
-		fill = fill + 1 == SLABS ? 0 : fill + 1;
+		begin();
+#pragma unroll
+		for (int l = 0; l < 2 * LOADS; ++l) { issue(fill, l); }
+		done();
 	};
-	for (int k = 0; k < SLABS - 1; ++k) { next(); }
-	for (uint32_t s = 0; s < g.slabs;)
+	for (int k = 0; k < SLABS - 2; ++k) { whole(); }
+	landed(); // the first slab
+	whole();
+	Half even, odd;
+#pragma unroll
+	for (int n = 0; n < READS; ++n) { read(even, 0, 0, n); }
+	// reads go out with the first two thirds of the products, loads with all of them
+	constexpr int FIRST = PRODUCTS * 2 / 3;
+	for (uint32_t s = 0; s < slabs;)
 	{
-		const uint32_t stop = CUT && s + g.cut < g.slabs ? s + g.cut : g.slabs;
+		const uint32_t stop = CUT && s + g.cut < slabs ? s + g.cut : slabs;
 		for (; s < stop; ++s)
 		{
+			multiply(even, [&] (int m)
+			{
+#pragma unroll
+				for (int n = 0; n < READS; ++n) { if (n * FIRST / READS == m) { read(odd, use, 1, n); } }
+			});
 			landed();
-			next();
-			multiply(use);
+			begin();
 			use = use + 1 == SLABS ? 0 : use + 1;
+			multiply(odd, [&] (int m)
+			{
+#pragma unroll
+				for (int n = 0; n < READS; ++n) { if (n * FIRST / READS == m) { read(even, use, 0, n); } }
+#pragma unroll
+				for (int l = 0; l < 2 * LOADS; ++l) { if (l * PRODUCTS / (2 * LOADS) == m) { issue(fill, l); } }
+			});
+			done();
 		}
 		if constexpr (CUT)
 		{
@@ -375,101 +407,109 @@ __global__ __launch_bounds__(256, 2) void ortho_pair_k (PairArgs g)
 	// nothing is on its way any more, LDS is free for the result
 	__builtin_amdgcn_s_waitcnt(0x0070);
 	__syncthreads();
-
 	const uint32_t i0 = bi * TILE + wi * (32 * WT), j0 = bj * TILE + wj * (32 * WT);
-	// the wave's tile as hi | lo << 16, [i][j]
-	uint32_t* meet = reinterpret_cast<uint32_t*>(lds) + wave * (32 * WT) * (32 * WT);
+	// a block of 32 x 32 lies inside the padded result or outside
+	auto inside = [&] (int ti, int tj) { return i0 + ti * 32 < g.rows_p && j0 + tj * 32 < g.rows_q; };
+	const uint64_t first32 = batch * g.stride32 + lane * 4;
+	float4 add[WT][WT][4];
+	if constexpr (MODE != GRAM)
+	{
+#pragma unroll
+		for (int ti = 0; ti < WT; ++ti)
+		{
+#pragma unroll
+			for (int tj = 0; tj < WT; ++tj)
+			{
+				const float* from = g.add32 + first32 + place32(g.rows_p, i0 / 32 + ti, j0 / 32 + tj);
+#pragma unroll
+				for (int r = 0; r < 4; ++r) { if (inside(ti, tj)) { add[ti][tj][r] = *reinterpret_cast<const float4*>(from + r * 256); } }
+			}
+		}
+	}
+	// The wave's tile by way of LDS, [i][j], as hi | lo << 16 (LAST: as it is): a store out of
+	// the registers would be 8 bytes in each of 32 rows, 20 us a tile of 192 x 192
+	constexpr uint32_t PITCH = 32 * WT + 1;
+	uint32_t* meet = reinterpret_cast<uint32_t*>(lds) + wave * (32 * WT) * PITCH;
 #pragma unroll
 	for (int ti = 0; ti < WT; ++ti)
 	{
 #pragma unroll
 		for (int tj = 0; tj < WT; ++tj)
 		{
+			if (!inside(ti, tj)) { continue; }
 			const f32x16 c = CUT ? sum[ti][tj] : acc[ti][tj];
-			const uint32_t j = j0 + tj * 32 + l32;
+			float* out32 = nullptr;
+			if constexpr (MODE == GRAM || MODE == APPLY) { out32 = g.out32 + first32 + place32(g.rows_p, i0 / 32 + ti, j0 / 32 + tj); }
 #pragma unroll
 			for (int r = 0; r < 4; ++r)
 			{
-				// four neighbouring rows of column j
-				const uint32_t i = i0 + ti * 32 + 8 * r + 4 * half;
-				const uint64_t place = (uint64_t) (i / 32) * BLOCK + i % 32;
-				float v[4];
-#pragma unroll
-				for (int e = 0; e < 4; ++e) { v[e] = c[4 * r + e] * g.alpha; }
-				if constexpr (CUT)
+				float4 v = make_float4(c[4 * r] * g.alpha, c[4 * r + 1] * g.alpha, c[4 * r + 2] * g.alpha, c[4 * r + 3] * g.alpha);
+				if constexpr (MODE != GRAM)
 				{
-					const uint64_t where = batch * g.stride_add + (uint64_t) j * g.ldadd + i;
-					const float4 x = *reinterpret_cast<const float4*>(g.add32 + where);
-					v[0] += x.x * g.beta; v[1] += x.y * g.beta; v[2] += x.z * g.beta; v[3] += x.w * g.beta;
-					if constexpr (MODE == APPLY) { *reinterpret_cast<float4*>(g.out_t32 + where) = make_float4(v[0], v[1], v[2], v[3]); }
+					const float4 x = add[ti][tj][r];
+					v.x += x.x * g.beta; v.y += x.y * g.beta; v.z += x.z * g.beta; v.w += x.w * g.beta;
 				}
-				else if constexpr (MODE == FACTOR)
+				if constexpr (MODE == GRAM || MODE == APPLY) { *reinterpret_cast<float4*>(out32 + r * 256) = v; }
+				const float w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+				for (int e = 0; e < 4; ++e)
 				{
-					const f16* add = g.add + batch * g.stride_add + (uint64_t) j * g.ldadd + place;
-					const f16x4 hi = *reinterpret_cast<const f16x4*>(add), lo = *reinterpret_cast<const f16x4*>(add + 32);
-#pragma unroll
-					for (int e = 0; e < 4; ++e) { v[e] += ((float) hi[e] + (float) lo[e]) * g.beta; }
-				}
-				if constexpr (MODE == LAST)
-				{
-					float* last = g.last + batch * g.stride_l;
-					if (j < g.n)
-					{
-						if (g.tall)
-						{
-							float* p = last + (uint64_t) j * g.ldl + i;
-							if (i + 4 <= g.m) { *reinterpret_cast<f32x4_any*>(p) = f32x4_any{v[0], v[1], v[2], v[3]}; }
-							else
-							{
-#pragma unroll
-								for (int e = 0; e < 4; ++e) { if (i + e < g.m) { p[e] = v[e]; } }
-							}
-						}
-						else
-						{
-#pragma unroll
-							for (int e = 0; e < 4; ++e) { if (i + e < g.m) { last[(uint64_t) (i + e) * g.ldl + j] = v[e]; } }
-						}
-					}
-				}
-				else
-				{
-					f16x4 hi, lo;
-#pragma unroll
-					for (int e = 0; e < 4; ++e)
-					{
-						const Split s = split(v[e]);
-						hi[e] = s.hi;
-						lo[e] = s.lo;
-						meet[(ti * 32 + 8 * r + 4 * half + e) * (32 * WT) + tj * 32 + l32] =
-							(uint32_t) __builtin_bit_cast(uint16_t, s.hi) | (uint32_t) __builtin_bit_cast(uint16_t, s.lo) << 16;
-					}
-					f16* out = g.out_t + batch * g.stride_ot + (uint64_t) j * g.ldot + place;
-					*reinterpret_cast<f16x4*>(out) = hi;
-					*reinterpret_cast<f16x4*>(out + 32) = lo;
+					meet[(ti * 32 + 8 * r + 4 * half + e) * PITCH + tj * 32 + l32] = MODE == LAST ? __builtin_bit_cast(uint32_t, w[e]) : packed(split(w[e]));
 				}
 			}
 		}
 	}
-	if constexpr (MODE != LAST)
+	// the wave reads what it wrote itself
+	__builtin_amdgcn_s_waitcnt(0xc07f); // lgkmcnt(0)
+	__builtin_amdgcn_wave_barrier();
+	constexpr uint32_t QUADS = 8 * WT; // groups of four along a row
+	// row `major` of the wave's tile (of its transposed: across), four elements from `minor` on
+	auto four = [&] (uint32_t major, uint32_t minor, bool across)
 	{
-		// a tile on the diagonal of a symmetric result is complete
-		if (SYMMETRIC && bi == bj) { return; }
-		// the wave reads what it wrote itself
-		__builtin_amdgcn_s_waitcnt(0xc07f); // lgkmcnt(0)
-		__builtin_amdgcn_wave_barrier();
-		constexpr uint32_t QUADS = 8 * WT; // a row's groups of four
+		const uint32_t* p = across ? meet + minor * PITCH + major : meet + major * PITCH + minor;
+		const uint32_t step = across ? PITCH : 1;
+		return make_uint4(p[0], p[step], p[2 * step], p[3 * step]);
+	};
+	auto store = [&] (f16* to, uint64_t ld, uint32_t major0, uint32_t minor0, uint32_t majors, uint32_t minors, bool across)
+	{
 #pragma unroll 4
 		for (uint32_t t = 0; t < 32 * WT * QUADS / TCG_WAVE; ++t)
 		{
-			const uint32_t e = t * TCG_WAVE + lane, i = e / QUADS, j = e % QUADS * 4;
-			const uint4 v = *reinterpret_cast<const uint4*>(meet + i * (32 * WT) + j);
+			const uint32_t e = t * TCG_WAVE + lane, major = e / QUADS, minor = e % QUADS * 4;
+			if (major0 + major >= majors || minor0 + minor >= minors) { continue; }
+			const uint4 v = four(major, minor, across);
 			uint2 hi, lo;
 			hi.x = (v.x & 0xffff) | v.y << 16; hi.y = (v.z & 0xffff) | v.w << 16;
 			lo.x = v.x >> 16 | (v.y & 0xffff0000u); lo.y = v.z >> 16 | (v.w & 0xffff0000u);
-			f16* out = g.out + batch * g.stride_o + (uint64_t) (i0 + i) * g.ldo + (uint64_t) ((j0 + j) / 32) * BLOCK + (j0 + j) % 32;
-			*reinterpret_cast<uint2*>(out) = hi;
-			*reinterpret_cast<uint2*>(out + 32) = lo;
+			f16* p = to + (uint64_t) (major0 + major) * ld + (uint64_t) ((minor0 + minor) / 32) * BLOCK + (minor0 + minor) % 32;
+			*reinterpret_cast<uint2*>(p) = hi;
+			*reinterpret_cast<uint2*>(p + 32) = lo;
+		}
+	};
+	if constexpr (MODE != LAST)
+	{
+		store(g.out_t + batch * g.stride_ot, g.ldot, j0, i0, g.rows_q, g.rows_p, true);
+		// a tile on the diagonal of a symmetric result is complete
+		if (SYMMETRIC && bi == bj) { return; }
+		store(g.out + batch * g.stride_o, g.ldo, i0, j0, g.rows_p, g.rows_q, false);
+	}
+	else
+	{
+		const uint32_t major0 = g.tall ? j0 : i0, minor0 = g.tall ? i0 : j0, majors = g.tall ? g.n : g.m, minors = g.tall ? g.m : g.n;
+#pragma unroll 4
+		for (uint32_t t = 0; t < 32 * WT * QUADS / TCG_WAVE; ++t)
+		{
+			const uint32_t e = t * TCG_WAVE + lane, major = e / QUADS, minor = e % QUADS * 4;
+			if (major0 + major >= majors || minor0 + minor >= minors) { continue; }
+			const uint4 v = four(major, minor, g.tall);
+			float* p = g.last + batch * g.stride_l + (uint64_t) (major0 + major) * g.ldl + minor0 + minor;
+			const float w[4] = {__builtin_bit_cast(float, v.x), __builtin_bit_cast(float, v.y), __builtin_bit_cast(float, v.z), __builtin_bit_cast(float, v.w)};
+			if (minor0 + minor + 4 <= minors) { *reinterpret_cast<f32x4_any*>(p) = f32x4_any{w[0], w[1], w[2], w[3]}; }
+			else
+			{
+#pragma unroll
+				for (int k = 0; k < 4; ++k) { if (minor0 + minor + k < minors) { p[k] = w[k]; } }
+			}
 		}
 	}
 }
@@ -527,11 +567,6 @@ __device__ __forceinline__ void small_product (f32x16& acc, const char* P, uint3
 			acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
 		}
 	}
-}
-
-__device__ __forceinline__ uint32_t packed (Split s)
-{
-	return (uint32_t) __builtin_bit_cast(uint16_t, s.hi) | (uint32_t) __builtin_bit_cast(uint16_t, s.lo) << 16;
 }
 
 template <int MT, int TILES>
@@ -937,14 +972,15 @@ float scale_of (double top)
 	return std::ldexp(1.f, 15 - e);
 }
 
-/// A slab is six additions to a sum; cut so that a part and the sum of the parts are
-/// chains of about one length.  Distance from the formulas at 768 rows (24 slabs):
-/// cut every 2 slabs 2.9e-6, every 8 3.6e-6; at 4096 (128 slabs): every 2 4.3e-6,
-/// every 8 3.1e-6; fp32 products that are never cut 1.3e-5 and 2.9e-5
+/// A slab is six additions to a sum; cut so that neither a part nor the sum of the parts
+/// is a long chain.  Distance from the formulas at 768 rows (24 slabs): cut every 2 or
+/// 4 slabs 2.9e-6, every 8 3.6e-6; at 4096 (128 slabs): every 2 4.3e-6, every 9 3.2e-6;
+/// fp32 products that are never cut 1.3e-5 and 2.9e-5.  A cut of a tile of 192 x 192 is
+/// 3900 cycles, two slabs' worth.
 uint32_t sum_cut (uint32_t slabs)
 {
-	const uint32_t cut = (uint32_t) std::lround(std::sqrt(slabs / 6.));
-	return cut < 2 ? 2 : cut;
+	const uint32_t cut = (uint32_t) std::lround(2 * std::sqrt(slabs / 6.));
+	return cut < 4 ? 4 : cut;
 }
 
 uint64_t padded (uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
@@ -970,14 +1006,56 @@ hipError_t pair_launch (tcg_ctx* ctx, const PairArgs& g, uint64_t batch)
 }
 
 template <int WT, int SLABS>
-hipError_t pair_launch_mode (tcg_ctx* ctx, Product mode, const PairArgs& g, uint64_t batch)
+hipError_t pair_launch_mode (tcg_ctx* ctx, Product mode, PairArgs& g, uint64_t batch)
 {
+	g.tiles_m = (g.rows_p + 64 * WT - 1) / (64 * WT);
+	g.tiles_n = (g.rows_q + 64 * WT - 1) / (64 * WT);
+	g.tiles = mode == GRAM || mode == FACTOR ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
 	switch (mode)
 	{
 		case GRAM: return pair_launch<WT,SLABS,GRAM>(ctx, g, batch);
 		case FACTOR: return pair_launch<WT,SLABS,FACTOR>(ctx, g, batch);
 		case APPLY: return pair_launch<WT,SLABS,APPLY>(ctx, g, batch);
 		default: return pair_launch<WT,SLABS,LAST>(ctx, g, batch);
+	}
+}
+
+// How a product is cut up.  Measured in cycles on this chip (tiles of 64 WT rows and
+// columns; a workgroup takes slabs x `slab` + `ends`, with `apply` instead of `slab`
+// where sums are cut and X is added):
+//   WT 1  five slabs in LDS, two workgroups a CU     slab 500 alone, 800 together, apply 900   ends 7000
+//   WT 2  four slabs, one workgroup a CU             slab 950                      apply 1400  ends 9000
+//   WT 3  three slabs, one workgroup a CU            slab 2030                     apply 2600  ends 16000
+// A larger tile reads less per product (WT 1 is bound by LDS, 48 KiB a slab for 200
+// cycles of matrix instructions; WT 3 keeps them busy 85 % of the time) and leaves
+// more of the chip idle in its last round.  4096 x 4096, all five steps: 6.6 ms with
+// WT 1, 5.6 with WT 2, 4.0 with WT 3; 1024 x 1024: 192, 429 and 740 us.
+struct PairCost
+{
+	uint32_t per_cu;
+	double slab, apply, ends;
+};
+constexpr PairCost pair_costs[4] = {{}, {2, 800, 900, 7000}, {1, 950, 1400, 9000}, {1, 2030, 2600, 16000}};
+
+/// Cycles of one product with tiles of 64 wt
+double pair_cycles (const tcg_ctx* ctx, int wt, bool symmetric, uint64_t rows_p, uint64_t rows_q, uint64_t slabs, uint64_t batch)
+{
+	const PairCost& c = pair_costs[wt];
+	const uint64_t tm = (rows_p + 64 * wt - 1) / (64 * wt), tn = (rows_q + 64 * wt - 1) / (64 * wt);
+	const uint64_t tiles = (symmetric ? tm * (tm + 1) / 2 : tm * tn) * batch;
+	const uint64_t room = (uint64_t) ctx->num_cus * c.per_cu;
+	double slab = symmetric ? c.slab : c.apply;
+	if (wt == 1 && tiles <= (uint64_t) ctx->num_cus) { slab = symmetric ? 500 : 650; }
+	return (double) ((tiles + room - 1) / room) * ((double) slabs * slab + c.ends);
+}
+
+hipError_t pair_dispatch (tcg_ctx* ctx, Product mode, int wt, PairArgs& g, uint64_t batch)
+{
+	switch (wt)
+	{
+		case 1: return pair_launch_mode<1,5>(ctx, mode, g, batch);
+		case 2: return pair_launch_mode<2,4>(ctx, mode, g, batch);
+		default: return pair_launch_mode<3,3>(ctx, mode, g, batch);
 	}
 }
 
@@ -1055,39 +1133,36 @@ int ortho_float (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, u
 	{
 		return ortho_small(ctx, plan, rows, cols, batch, in, ldg, stride_g, eps, out, ldo, stride_o, tiles);
 	}
-	// tiles of 128 x 128 where they fill the chip, of 64 x 64 elsewhere
-	const uint64_t big = padded(m, 128) / 128 * (padded(n, 128) / 128) * batch;
-	const int wt = big >= (uint64_t) ctx->num_cus ? 2 : 1;
-	const uint64_t tile = 64 * wt, mp = padded(m, tile), np = padded(n, tile);
-	const uint32_t tm = (uint32_t) (mp / tile), tn = (uint32_t) (np / tile);
-	TCG_REQUIRE(ctx, (uint64_t) tm * tn * batch < (1ull << 31), "tcg_orthogonalize: %llu matrices of %llu x %llu are too many",
+	const uint64_t mp = padded(m, 64), np = padded(n, 64);
+	TCG_REQUIRE(ctx, mp / 64 * (np / 64) * batch < (1ull << 31), "tcg_orthogonalize: %llu matrices of %llu x %llu are too many",
 		(unsigned long long) batch, (unsigned long long) rows, (unsigned long long) cols);
-	// X, X^T and X^T in fp32 before and after a step, A, B; 32 bits an element each
+	// X, X^T and X in fp32 before and after a step, A, A in fp32, B; 32 bits an element each
 	const size_t xs = (size_t) mp * np * 2, as = (size_t) mp * mp * 2; // halves
 	const uint32_t parts = norm_parts(rows);
 	const size_t sums_bytes = ((size_t) batch * parts * sizeof(double) + 255) / 256 * 256;
-	const size_t bytes = sums_bytes + (6 * xs + 2 * as) * batch * sizeof(f16);
+	const size_t bytes = sums_bytes + (6 * xs + 3 * as) * batch * sizeof(f16);
 	void* mem = nullptr;
 	int rc = tcg_alloc(ctx, bytes, &mem);
 	if (rc != TCG_OK) { return rc; }
 	f16* x[2], *xt[2];
-	float* xt32[2];
+	float* x32[2];
 	f16* p = reinterpret_cast<f16*>((char*) mem + sums_bytes);
 	for (int k = 0; k < 2; ++k)
 	{
 		x[k] = p; p += xs * batch;
 		xt[k] = p; p += xs * batch;
-		xt32[k] = reinterpret_cast<float*>(p); p += xs * batch;
+		x32[k] = reinterpret_cast<float*>(p); p += xs * batch;
 	}
 	f16* gram = p;
 	f16* factor = gram + as * batch;
+	float* gram32 = reinterpret_cast<float*>(factor + as * batch);
 
 	PrepArgs<float> prep = {};
 	prep.g = in; prep.ldg = ldg; prep.stride_g = stride_g;
 	prep.rows = rows; prep.cols = cols;
 	prep.parts = parts; prep.sums = (double*) mem; prep.eps = eps;
 	prep.scale = scale_of(plan.x[0]);
-	prep.x = x[0]; prep.xt = xt[0]; prep.xt32 = xt32[0];
+	prep.x = x[0]; prep.xt = xt[0]; prep.x32 = x32[0];
 	prep.ldx = np * 2; prep.ldxt = mp * 2;
 	prep.stride_x = prep.stride_xt = xs;
 	prep.tall = tall;
@@ -1095,28 +1170,39 @@ int ortho_float (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, u
 	const uint32_t tiles_x = (uint32_t) ((tall ? mp : np) / 64);
 	ortho_split_k<<<dim3((unsigned) (mp / 64 * (np / 64)), (unsigned) batch), 256, 0, ctx->stream>>>(prep, tiles_x);
 
+	// A in fp32 goes from GRAM to FACTOR in the order of their tiles: one size for both
+	int wt_gram = 1, wt_apply = 1;
+	double least_gram = 1e300, least_apply = 1e300;
+	for (int wt = 1; wt <= 3; ++wt)
+	{
+		const double both = pair_cycles(ctx, wt, true, mp, mp, np / 32, batch) + pair_cycles(ctx, wt, true, mp, mp, mp / 32, batch);
+		const double apply = pair_cycles(ctx, wt, false, mp, np, mp / 32, batch);
+		if (both < least_gram) { least_gram = both; wt_gram = wt; }
+		if (apply < least_apply) { least_apply = apply; wt_apply = wt; }
+	}
 	hipError_t err = hipGetLastError();
-	auto launch = [&] (Product mode, const PairArgs& g)
+	auto launch = [&] (Product mode, PairArgs& g)
 	{
 		if (err != hipSuccess) { return; }
-		err = wt == 2 ? pair_launch_mode<2,2>(ctx, mode, g, batch) : pair_launch_mode<1,4>(ctx, mode, g, batch);
+		err = pair_dispatch(ctx, mode, mode == GRAM || mode == FACTOR ? wt_gram : wt_apply, g, batch);
 	};
 	for (int k = 0; k < plan.steps; ++k)
 	{
 		const int now = k & 1, next = now ^ 1;
 		const float sx = scale_of(plan.x[k]), sa = scale_of(plan.gram[k]), sb = scale_of(plan.factor[k]);
 		PairArgs g = {};
-		g.tiles_m = g.tiles_n = tm;
-		g.tiles = tm * (tm + 1) / 2;
+		g.rows_p = g.rows_q = (uint32_t) mp;
 		g.p = g.q = x[now];
 		g.ldp = g.ldq = np * 2; g.stride_p = g.stride_q = xs;
 		g.slabs = (uint32_t) (np / 32);
 		g.alpha = sa / sx / sx;
+		g.out32 = gram32; g.stride32 = as / 2;
 		g.out = g.out_t = gram;
 		g.ldo = g.ldot = mp * 2; g.stride_o = g.stride_ot = as;
 		launch(GRAM, g);
-		g.p = g.q = g.add = gram;
-		g.ldp = g.ldq = g.ldadd = mp * 2; g.stride_p = g.stride_q = g.stride_add = as;
+		g.p = g.q = gram;
+		g.ldp = g.ldq = mp * 2; g.stride_p = g.stride_q = as;
+		g.add32 = gram32; g.out32 = nullptr;
 		g.slabs = (uint32_t) (mp / 32);
 		g.alpha = (float) plan.c * (sb / sa / sa);
 		g.beta = (float) plan.b * (sb / sa);
@@ -1124,13 +1210,11 @@ int ortho_float (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, u
 		launch(FACTOR, g);
 		const bool last = k + 1 == plan.steps;
 		const float sn = last ? 1.f : scale_of(plan.x[k + 1]);
-		g.tiles_n = tn;
-		g.tiles = tm * tn;
+		g.rows_q = (uint32_t) np;
 		g.p = factor;
 		g.q = xt[now];
 		g.ldq = mp * 2; g.stride_q = xs;
-		g.add32 = xt32[now]; g.out_t32 = xt32[next];
-		g.ldadd = mp; g.stride_add = xs / 2;
+		g.add32 = x32[now]; g.out32 = x32[next]; g.stride32 = xs / 2;
 		g.cut = sum_cut(g.slabs);
 		g.alpha = sn / sb / sx;
 		g.beta = (float) plan.a * (sn / sx);
