@@ -761,15 +761,14 @@ __global__ __launch_bounds__(1024) void ortho_small_k (SmallArgs g)
 
 // ---- double -----------------------------------------------------------------------------
 // The same steps over dense doubles, padded with zeros to multiples of 64 rows and
-// columns, both operands with the summed index along memory.  A wave holds a 32 x 32
-// tile (v_mfma_f64_16x16x4: lane i + 16 q supplies element (i, q) of an operand and
-// holds elements (4 r + q, i) of the result) and reads its operands straight from
-// memory, 16 bytes a lane: the matrix instructions take 32 cycles each, eight of
-// them for four loads, so the loads of the next indices are out long before they
-// are used and nothing has to be staged.  KSPLIT = 4: the four waves of a workgroup
-// share one tile, every fourth group of eight summed indices each, and their parts
-// are added in wave order (few tiles); KSPLIT = 1: a wave to each quarter of a 64 x 64
-// tile (the operands are read half as often).
+// columns, both operands with the summed index along memory.  A wave holds TI x TI
+// blocks of 16 x 16 (v_mfma_f64_16x16x4: lane i + 16 q supplies element (i, q) of an
+// operand and holds elements (4 r + q, i) of the result) and reads its operands straight
+// from memory, three groups of eight summed indices ahead: a matrix instruction takes
+// 64 cycles, so nothing has to be staged.  KSPLIT = 4: the four waves
+// of a workgroup share one tile, every fourth group each, and their parts are added in
+// wave order; KSPLIT = 1: a wave to each quarter of a 64 x 64 tile (the operands are read
+// half as often as with tiles of 32).
 
 typedef double f64x2 __attribute__((ext_vector_type(2)));
 typedef double f64x4 __attribute__((ext_vector_type(4)));
@@ -794,11 +793,12 @@ struct DoubleArgs
 	bool tall;
 };
 
-template <int KSPLIT, int MODE>
+template <int KSPLIT, int TI, int MODE>
 __global__ __launch_bounds__(256) void ortho_double_k (DoubleArgs g)
 {
 	constexpr bool SYMMETRIC = MODE == GRAM || MODE == FACTOR;
-	constexpr uint32_t TILE = KSPLIT == 1 ? 64 : 32;
+	static_assert(KSPLIT == 4 || (KSPLIT == 1 && TI == 2), "four waves share a tile, or hold a quarter of one each");
+	constexpr uint32_t WAVE_TILE = 16 * TI, TILE = KSPLIT == 1 ? 64 : WAVE_TILE;
 	constexpr uint32_t PITCH = TILE + 1;
 	__shared__ double meet[KSPLIT * TILE * PITCH];
 	const uint32_t total = gridDim.x, xcd = blockIdx.x % 8, each = total / 8, more = total % 8;
@@ -814,76 +814,108 @@ __global__ __launch_bounds__(256) void ortho_double_k (DoubleArgs g)
 	const uint32_t wave = threadIdx.x / TCG_WAVE, lane = threadIdx.x & (TCG_WAVE - 1);
 	const uint32_t l16 = lane & 15, quarter = lane >> 4;
 	const uint32_t wi = KSPLIT == 1 ? wave / 2 : 0, wj = KSPLIT == 1 ? wave % 2 : 0;
-	const double* p = g.p + batch * g.stride_p + (uint64_t) (bi * TILE + wi * 32 + l16) * g.ldp + 2 * quarter;
-	const double* q = g.q + batch * g.stride_q + (uint64_t) (bj * TILE + wj * 32 + l16) * g.ldq + 2 * quarter;
-	f64x4 acc[2][2] = {};
-	constexpr uint32_t STEP = KSPLIT == 1 ? 8 : 32; // between a wave's groups of eight indices
-	constexpr uint32_t AHEAD = 2;                   // groups loaded together
-	for (uint32_t k = KSPLIT == 1 ? 0 : wave * 8; k < g.depth; k += STEP * AHEAD)
+	const double* p = g.p + batch * g.stride_p + (uint64_t) (bi * TILE + wi * WAVE_TILE + l16) * g.ldp + 2 * quarter;
+	const double* q = g.q + batch * g.stride_q + (uint64_t) (bj * TILE + wj * WAVE_TILE + l16) * g.ldq + 2 * quarter;
+	const uint32_t i0 = bi * TILE, j0 = bj * TILE;
+	// what C is added to, ahead of everything: its loads would wait for each other's stores
+	constexpr uint32_t EACH = TILE * TILE / 256;
+	double add[EACH];
+#pragma unroll
+	for (uint32_t t = 0; t < EACH; ++t)
 	{
-		f64x2 a[AHEAD][2], b[AHEAD][2];
+		const uint32_t e = t * 256 + threadIdx.x;
+		add[t] = MODE == GRAM ? 0 : g.add[batch * g.stride_add + (uint64_t) (i0 + e / TILE) * g.ldadd + j0 + e % TILE];
+	}
+	f64x4 acc[TI][TI] = {};
+	constexpr uint32_t STEP = 8 * KSPLIT; // between a wave's groups of eight indices
+	const uint32_t groups = g.depth / STEP, first = KSPLIT == 1 ? 0 : wave * 8;
+	struct Group
+	{
+		f64x2 a[TI], b[TI];
+	};
+	Group ring[4];
+	auto load = [&] (Group& to, uint32_t n)
+	{
+		const uint32_t k = first + (n < groups ? n : groups - 1) * STEP;
 #pragma unroll
-		for (uint32_t h = 0; h < AHEAD; ++h)
+		for (int t = 0; t < TI; ++t)
 		{
-#pragma unroll
-			for (int t = 0; t < 2; ++t)
-			{
-				a[h][t] = *reinterpret_cast<const f64x2*>(p + (uint64_t) t * 16 * g.ldp + k + h * STEP);
-				b[h][t] = *reinterpret_cast<const f64x2*>(q + (uint64_t) t * 16 * g.ldq + k + h * STEP);
-			}
+			to.a[t] = *reinterpret_cast<const f64x2*>(p + (uint64_t) t * 16 * g.ldp + k);
+			to.b[t] = *reinterpret_cast<const f64x2*>(q + (uint64_t) t * 16 * g.ldq + k);
 		}
+	};
+	auto multiply = [&] (const Group& x)
+	{
 #pragma unroll
-		for (uint32_t h = 0; h < AHEAD; ++h)
+		for (int e = 0; e < 2; ++e)
 		{
 #pragma unroll
-			for (int e = 0; e < 2; ++e)
+			for (int i = 0; i < TI; ++i)
 			{
 #pragma unroll
-				for (int i = 0; i < 2; ++i)
+				for (int j = 0; j < TI; ++j)
 				{
-#pragma unroll
-					for (int j = 0; j < 2; ++j)
-					{
-						acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64(a[h][i][e], b[h][j][e], acc[i][j], 0, 0, 0);
-					}
+					acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64(x.a[i][e], x.b[j][e], acc[i][j], 0, 0, 0);
 				}
 			}
 		}
+	};
+#pragma unroll
+	for (uint32_t u = 0; u < 3; ++u) { load(ring[u], u); }
+	uint32_t n = 0;
+	// four groups at a time without a branch between them: with one the compiler waits for
+	// every load that is out
+	for (; n + 4 <= groups; n += 4)
+	{
+#pragma unroll
+		for (uint32_t u = 0; u < 4; ++u)
+		{
+			load(ring[(u + 3) % 4], n + u + 3);
+			__builtin_amdgcn_sched_barrier(0);
+			multiply(ring[u]);
+			__builtin_amdgcn_sched_barrier(0);
+		}
+	}
+#pragma unroll
+	for (uint32_t u = 0; u < 3; ++u)
+	{
+		if (n + u < groups) { multiply(ring[u]); }
 	}
 	double* mine = meet + (KSPLIT == 1 ? 0 : wave * TILE * PITCH);
 #pragma unroll
-	for (int i = 0; i < 2; ++i)
+	for (int i = 0; i < TI; ++i)
 	{
 #pragma unroll
-		for (int j = 0; j < 2; ++j)
+		for (int j = 0; j < TI; ++j)
 		{
 #pragma unroll
 			for (int r = 0; r < 4; ++r)
 			{
-				mine[(wi * 32 + i * 16 + 4 * r + quarter) * PITCH + wj * 32 + j * 16 + l16] = acc[i][j][r];
+				mine[(wi * WAVE_TILE + i * 16 + 4 * r + quarter) * PITCH + wj * WAVE_TILE + j * 16 + l16] = acc[i][j][r];
 			}
 		}
 	}
 	__syncthreads();
-	const uint32_t i0 = bi * TILE, j0 = bj * TILE;
 	// the result where its rows run along memory; what is kept transposed goes by LDS
-	for (uint32_t e = threadIdx.x; e < TILE * TILE; e += 256)
+#pragma unroll
+	for (uint32_t t = 0; t < EACH; ++t)
 	{
-		const uint32_t i = e / TILE, j = e % TILE;
+		const uint32_t e = t * 256 + threadIdx.x, i = e / TILE, j = e % TILE;
 		double v = 0;
 #pragma unroll
 		for (int w = 0; w < KSPLIT; ++w) { v += meet[w * TILE * PITCH + i * PITCH + j]; }
 		v *= g.alpha;
-		if constexpr (MODE != GRAM) { v += g.beta * g.add[batch * g.stride_add + (uint64_t) (i0 + i) * g.ldadd + j0 + j]; }
+		if constexpr (MODE != GRAM) { v += g.beta * add[t]; }
 		if constexpr (MODE != LAST) { g.out[batch * g.stride_o + (uint64_t) (i0 + i) * g.ldo + j0 + j] = v; }
 		else if (!g.tall && i0 + i < g.m && j0 + j < g.n) { g.last[batch * g.stride_l + (uint64_t) (i0 + i) * g.ldl + j0 + j] = v; }
 		meet[i * PITCH + j] = v; // read by this lane alone until now
 	}
 	__syncthreads();
 	if ((SYMMETRIC && bi == bj) || (MODE == LAST && !g.tall)) { return; }
-	for (uint32_t e = threadIdx.x; e < TILE * TILE; e += 256)
+#pragma unroll
+	for (uint32_t t = 0; t < EACH; ++t)
 	{
-		const uint32_t j = e / TILE, i = e % TILE;
+		const uint32_t e = t * 256 + threadIdx.x, j = e / TILE, i = e % TILE;
 		const double v = meet[i * PITCH + j];
 		if constexpr (MODE != LAST) { g.out_t[batch * g.stride_ot + (uint64_t) (j0 + j) * g.ldot + i0 + i] = v; }
 		else if (i0 + i < g.m && j0 + j < g.n) { g.last[batch * g.stride_l + (uint64_t) (j0 + j) * g.ldl + i0 + i] = v; }
@@ -1230,16 +1262,16 @@ int ortho_float (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, u
 	return rc;
 }
 
-template <int KSPLIT>
+template <int KSPLIT, int TI>
 void double_launch (tcg_ctx* ctx, Product mode, const DoubleArgs& g, uint64_t batch)
 {
 	const unsigned grid = (unsigned) (g.tiles * batch);
 	switch (mode)
 	{
-		case GRAM: ortho_double_k<KSPLIT,GRAM><<<grid, 256, 0, ctx->stream>>>(g); break;
-		case FACTOR: ortho_double_k<KSPLIT,FACTOR><<<grid, 256, 0, ctx->stream>>>(g); break;
-		case APPLY: ortho_double_k<KSPLIT,APPLY><<<grid, 256, 0, ctx->stream>>>(g); break;
-		default: ortho_double_k<KSPLIT,LAST><<<grid, 256, 0, ctx->stream>>>(g); break;
+		case GRAM: ortho_double_k<KSPLIT,TI,GRAM><<<grid, 256, 0, ctx->stream>>>(g); break;
+		case FACTOR: ortho_double_k<KSPLIT,TI,FACTOR><<<grid, 256, 0, ctx->stream>>>(g); break;
+		case APPLY: ortho_double_k<KSPLIT,TI,APPLY><<<grid, 256, 0, ctx->stream>>>(g); break;
+		default: ortho_double_k<KSPLIT,TI,LAST><<<grid, 256, 0, ctx->stream>>>(g); break;
 	}
 }
 
@@ -1253,7 +1285,7 @@ int ortho_double (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, 
 	const uint32_t parts = norm_parts(rows);
 	const size_t sums_bytes = ((size_t) batch * parts * sizeof(double) + 255) / 256 * 256;
 	const size_t bytes = sums_bytes + (4 * xs + 2 * as) * batch * sizeof(double);
-	TCG_REQUIRE(ctx, mp / 32 * (np / 32) * batch < (1ull << 31), "tcg_orthogonalize: %llu matrices of %llu x %llu are too many",
+	TCG_REQUIRE(ctx, mp / 16 * (np / 16) * batch < (1ull << 31), "tcg_orthogonalize: %llu matrices of %llu x %llu are too many",
 		(unsigned long long) batch, (unsigned long long) rows, (unsigned long long) cols);
 	void* mem = nullptr;
 	int rc = tcg_alloc(ctx, bytes, &mem);
@@ -1273,16 +1305,28 @@ int ortho_double (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, 
 	prep.tall = tall;
 	ortho_norm_k<double><<<dim3(parts, (unsigned) batch), 256, 0, ctx->stream>>>(prep);
 	ortho_scale_k<<<dim3((unsigned) (mp / 64 * (np / 64)), (unsigned) batch), 256, 0, ctx->stream>>>(prep, (uint32_t) ((tall ? mp : np) / 64));
+	// Tiles of 64 where there are two for every CU, of 16 where tiles of 32 would leave half
+	// of the CUs without one (256 x 256: 127 us with tiles of 32, 85 with tiles of 16;
+	// 1024 x 1024: 840 us with tiles of 32, 1000 with tiles of 64, 1460 with tiles of 16)
 	auto launch = [&] (Product mode, DoubleArgs& g, uint64_t height, uint64_t width)
 	{
-		// 64 x 64 tiles where they fill the chip twice, else the summed index shared by the waves of a tile
-		const bool wide = height / 64 * (width / 64) * batch >= 2 * (uint64_t) ctx->num_cus;
-		const uint32_t tile = wide ? 64 : 32;
+		const bool symmetric = mode == GRAM || mode == FACTOR;
+		auto tiles = [&] (uint64_t tile)
+		{
+			const uint64_t tm = height / tile, tn = width / tile;
+			return symmetric ? tm * (tm + 1) / 2 : tm * tn;
+		};
+		const uint64_t cus = (uint64_t) ctx->num_cus;
+		const uint32_t tile = tiles(64) * batch >= 2 * cus ? 64 : 2 * tiles(32) * batch <= cus ? 16 : 32;
 		g.tiles_m = (uint32_t) (height / tile);
 		g.tiles_n = (uint32_t) (width / tile);
-		g.tiles = mode == GRAM || mode == FACTOR ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
-		if (wide) { double_launch<1>(ctx, mode, g, batch); }
-		else { double_launch<4>(ctx, mode, g, batch); }
+		g.tiles = (uint32_t) tiles(tile);
+		switch (tile)
+		{
+			case 64: double_launch<1,2>(ctx, mode, g, batch); break;
+			case 32: double_launch<4,2>(ctx, mode, g, batch); break;
+			default: double_launch<4,1>(ctx, mode, g, batch); break;
+		}
 	};
 	for (int k = 0; k < plan.steps; ++k)
 	{
