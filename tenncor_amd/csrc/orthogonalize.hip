@@ -75,6 +75,8 @@ struct PrepArgs
 	double* sums; // [batch][parts]
 	double eps;
 	float scale;
+	uint32_t* arrived; // [batch][arrivals], cleared here for the products that count in them
+	uint32_t arrivals;
 	// float: X and X^T as split matrices, padded; double: dense, padded
 	f16* x;
 	f16* xt;
@@ -116,6 +118,10 @@ __global__ __launch_bounds__(256) void ortho_norm_k (PrepArgs<T> a)
 			sum += v * v;
 		}
 	}
+	if (blockIdx.x == 0)
+	{
+		for (uint32_t i = threadIdx.x; i < a.arrivals; i += blockDim.x) { a.arrived[(uint64_t) blockIdx.y * a.arrivals + i] = 0; }
+	}
 	sum = group_sum(sum, red);
 	if (threadIdx.x == 0) { a.sums[(uint64_t) blockIdx.y * a.parts + blockIdx.x] = sum; }
 }
@@ -136,6 +142,26 @@ __device__ __forceinline__ uint64_t place32 (uint32_t rows, uint32_t bi, uint32_
 	return ((uint64_t) bj * (rows / 32) + bi) * 1024;
 }
 
+/// A thread's 16 values of the 64 x 64 tile of G at (r0, c0): rows threadIdx.x / 64 + 4 i of
+/// column threadIdx.x % 64, zero outside of G.  No branch around a load, so that all are on
+/// their way together (a branch each, waited for in turn: 13 us instead of 6 us at 768 x 2048)
+template <typename T>
+__device__ __forceinline__ void tile_values (T (&v)[16], const PrepArgs<T>& a, const T* g, uint64_t r0, uint64_t c0)
+{
+	const uint64_t col = c0 + threadIdx.x % 64, at = col < a.cols ? col : a.cols - 1;
+#pragma unroll
+	for (int i = 0; i < 16; ++i)
+	{
+		const uint64_t row = r0 + threadIdx.x / 64 + 4 * i;
+		v[i] = g[(row < a.rows ? row : a.rows - 1) * a.ldg + at];
+	}
+#pragma unroll
+	for (int i = 0; i < 16; ++i)
+	{
+		if (col >= a.cols || r0 + threadIdx.x / 64 + 4 * i >= a.rows) { v[i] = 0; }
+	}
+}
+
 // X = G / (|G| + eps) and X^T as split matrices, a 64 x 64 tile a workgroup; what
 // lies outside G is zero
 __global__ __launch_bounds__(256) void ortho_split_k (PrepArgs<float> a, uint32_t tiles_x)
@@ -143,24 +169,21 @@ __global__ __launch_bounds__(256) void ortho_split_k (PrepArgs<float> a, uint32_
 	__shared__ double red[4];
 	__shared__ float tile[64][65];
 	const uint32_t batch = blockIdx.y;
-	const double inv = inverse_norm(a, batch, red) * a.scale;
 	const uint64_t r0 = (uint64_t) (blockIdx.x / tiles_x) * 64, c0 = (uint64_t) (blockIdx.x % tiles_x) * 64;
-	const float* g = a.g + batch * a.stride_g;
-	for (uint32_t e = threadIdx.x; e < 64 * 64; e += 256)
-	{
-		const uint32_t r = e / 64, c = e % 64;
-		float v = 0;
-		if (r0 + r < a.rows && c0 + c < a.cols) { v = (float) ((double) g[(r0 + r) * a.ldg + c0 + c] * inv); }
-		tile[r][c] = v;
-	}
+	float v[16];
+	tile_values(v, a, a.g + batch * a.stride_g, r0, c0);
+	const double inv = inverse_norm(a, batch, red) * a.scale;
+#pragma unroll
+	for (int i = 0; i < 16; ++i) { tile[threadIdx.x / 64 + 4 * i][threadIdx.x % 64] = (float) ((double) v[i] * inv); }
 	__syncthreads();
 	// G's rows are X's rows, or X^T's
 	f16* along = (a.tall ? a.xt + batch * a.stride_xt : a.x + batch * a.stride_x);
 	f16* across = (a.tall ? a.x + batch * a.stride_x : a.xt + batch * a.stride_xt);
 	const uint64_t ld_along = a.tall ? a.ldxt : a.ldx, ld_across = a.tall ? a.ldx : a.ldxt;
-	for (uint32_t e = threadIdx.x; e < 64 * 16; e += 256)
+#pragma unroll
+	for (int k = 0; k < 4; ++k)
 	{
-		const uint32_t r = e / 16, c = e % 16 * 4;
+		const uint32_t r = threadIdx.x / 16 + 16 * k, c = threadIdx.x % 16 * 4;
 		f16x4 hi, lo, thi, tlo;
 #pragma unroll
 		for (int i = 0; i < 4; ++i)
@@ -203,6 +226,11 @@ struct PairArgs
 	uint32_t rows_p, rows_q; // padded to whole blocks of 32
 	uint32_t slabs; // of 32 summed indices
 	uint32_t cut;   // slabs between two cuts of the sums of B X
+	// GRAM: `parts` workgroups share a tile, `share` slabs each; their sums meet in `partial`
+	// [batch][tiles][parts][tile], and the last to arrive adds them up, in order
+	uint32_t parts, share;
+	float* partial;
+	uint32_t* arrived; // [batch][tiles], zero between two launches
 	uint32_t tiles_m, tiles_n, tiles; // tiles: of one matrix (one triangle of them for GRAM and FACTOR)
 	// C alpha + add beta, and that in fp32 as it is in the registers of the matrix
 	// instructions (`place32`): nothing but the next product of the same tiles reads it
@@ -247,12 +275,20 @@ __global__ __launch_bounds__(256) void ortho_pair_k (PairArgs g)
 	constexpr int LOADS = 2 * WT;       // a wave's loads per operand and slab
 	constexpr bool SYMMETRIC = MODE == GRAM || MODE == FACTOR;
 	constexpr bool CUT = MODE == APPLY || MODE == LAST;
+	constexpr bool SHARED = MODE == GRAM && WT == 1; // a larger tile has no need of it
 	extern __shared__ __attribute__((aligned(1024))) char lds[];
 
 	// consecutive workgroups go to the XCDs in turn: each XCD gets a run of
 	// neighbouring tiles, which share rows of P
 	const uint32_t total = gridDim.x, xcd = blockIdx.x % 8, each = total / 8, more = total % 8;
-	const uint32_t at = xcd * each + (xcd < more ? xcd : more) + blockIdx.x / 8;
+	uint32_t at = xcd * each + (xcd < more ? xcd : more) + blockIdx.x / 8;
+	uint32_t part = 0, slabs = g.slabs;
+	if constexpr (SHARED)
+	{
+		part = at % g.parts;
+		at /= g.parts;
+		slabs = slabs - part * g.share < g.share ? slabs - part * g.share : g.share;
+	}
 	const uint32_t batch = at / g.tiles;
 	const uint32_t tile = at % g.tiles;
 	uint32_t bi, bj;
@@ -278,8 +314,9 @@ __global__ __launch_bounds__(256) void ortho_pair_k (PairArgs g)
 		const uint32_t chunk = (lane & 7) ^ swizzle(r);
 		// rows past the end: the last one again, never stored
 		const uint32_t rp = bi * TILE + r, rq = bj * TILE + r;
-		from[0][i] = g.p + batch * g.stride_p + (uint64_t) (rp < g.rows_p ? rp : g.rows_p - 1) * g.ldp + chunk * 8;
-		from[1][i] = g.q + batch * g.stride_q + (uint64_t) (rq < g.rows_q ? rq : g.rows_q - 1) * g.ldq + chunk * 8;
+		const uint64_t first = SHARED ? (uint64_t) part * g.share * BLOCK : 0;
+		from[0][i] = g.p + batch * g.stride_p + (uint64_t) (rp < g.rows_p ? rp : g.rows_p - 1) * g.ldp + first + chunk * 8;
+		from[1][i] = g.q + batch * g.stride_q + (uint64_t) (rq < g.rows_q ? rq : g.rows_q - 1) * g.ldq + first + chunk * 8;
 		const uint32_t base = (uint32_t) (uintptr_t) (const __attribute__((address_space(3))) char*) lds + (wave * (16 * WT) + i * 8) * 128;
 		to[0][i] = __builtin_amdgcn_readfirstlane(base);
 		to[1][i] = __builtin_amdgcn_readfirstlane(base + OPERAND);
@@ -349,7 +386,6 @@ __global__ __launch_bounds__(256) void ortho_pair_k (PairArgs g)
 		__builtin_amdgcn_s_barrier();
 		__builtin_amdgcn_sched_barrier(0);
 	};
-	const uint32_t slabs = g.slabs;
 	uint32_t issued = 0, fill = 0, use = 0;
 	auto begin = [&] () { if (++issued >= slabs) { ahead = 0; } }; // stays at the last slab
 	auto done = [&] () { fill = fill + 1 == SLABS ? 0 : fill + 1; };
@@ -407,6 +443,42 @@ __global__ __launch_bounds__(256) void ortho_pair_k (PairArgs g)
 	// nothing is on its way any more, LDS is free for the result
 	__builtin_amdgcn_s_waitcnt(0x0070);
 	__syncthreads();
+	if constexpr (SHARED)
+	{
+		if (g.parts > 1)
+		{
+			// Stores and loads that pass the L2 of the XCD by, which is not coherent with the
+			// others': a fence, which writes all of that L2 back, took 25 us a product
+			uint64_t* mine = reinterpret_cast<uint64_t*>(g.partial + (uint64_t) at * g.parts * (TILE * TILE)) + threadIdx.x;
+#pragma unroll
+			for (int r = 0; r < 8; ++r)
+			{
+				__hip_atomic_store(mine + part * (TILE * TILE / 2) + r * 256, __builtin_bit_cast(uint64_t, make_float2(acc[0][0][2 * r], acc[0][0][2 * r + 1])),
+					__ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+			}
+			// they have arrived, those of every wave, before the workgroup counts
+			__builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+			__builtin_amdgcn_s_waitcnt(0x0070);
+			__syncthreads();
+			uint32_t* count = reinterpret_cast<uint32_t*>(lds);
+			if (threadIdx.x == 0) { *count = __hip_atomic_fetch_add(g.arrived + at, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+			__syncthreads();
+			if (*count + 1 != g.parts) { return; }
+			if (threadIdx.x == 0) { __hip_atomic_store(g.arrived + at, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+			f32x16 all = {};
+			for (uint32_t q = 0; q < g.parts; ++q)
+			{
+#pragma unroll
+				for (int r = 0; r < 8; ++r)
+				{
+					const float2 v = __builtin_bit_cast(float2, __hip_atomic_load(mine + q * (TILE * TILE / 2) + r * 256, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+					all[2 * r] += v.x; all[2 * r + 1] += v.y;
+				}
+			}
+			acc[0][0] = all;
+			__syncthreads(); // `count` lies where the result goes
+		}
+	}
 	const uint32_t i0 = bi * TILE + wi * (32 * WT), j0 = bj * TILE + wj * (32 * WT);
 	// a block of 32 x 32 lies inside the padded result or outside
 	auto inside = [&] (int ti, int tj) { return i0 + ti * 32 < g.rows_p && j0 + tj * 32 < g.rows_q; };
@@ -928,24 +1000,25 @@ __global__ __launch_bounds__(256) void ortho_scale_k (PrepArgs<double> a, uint32
 	__shared__ double red[4];
 	__shared__ double tile[64][65];
 	const uint32_t batch = blockIdx.y;
-	const double inv = inverse_norm(a, batch, red);
 	const uint64_t r0 = (uint64_t) (blockIdx.x / tiles_x) * 64, c0 = (uint64_t) (blockIdx.x % tiles_x) * 64;
-	const double* g = a.g + batch * a.stride_g;
+	double v[16];
+	tile_values(v, a, a.g + batch * a.stride_g, r0, c0);
+	const double inv = inverse_norm(a, batch, red);
 	double* along = a.dense[a.tall] + batch * a.stride_dense;
 	double* across = a.dense[!a.tall] + batch * a.stride_dense;
 	const uint64_t ld_along = a.tall ? a.ldxt : a.ldx, ld_across = a.tall ? a.ldx : a.ldxt;
-	for (uint32_t e = threadIdx.x; e < 64 * 64; e += 256)
+#pragma unroll
+	for (int i = 0; i < 16; ++i)
 	{
-		const uint32_t r = e / 64, c = e % 64;
-		double v = 0;
-		if (r0 + r < a.rows && c0 + c < a.cols) { v = g[(r0 + r) * a.ldg + c0 + c] * inv; }
-		tile[r][c] = v;
-		along[(r0 + r) * ld_along + c0 + c] = v;
+		const uint32_t r = threadIdx.x / 64 + 4 * i, c = threadIdx.x % 64;
+		tile[r][c] = v[i] * inv;
+		along[(r0 + r) * ld_along + c0 + c] = v[i] * inv;
 	}
 	__syncthreads();
-	for (uint32_t e = threadIdx.x; e < 64 * 64; e += 256)
+#pragma unroll
+	for (int i = 0; i < 16; ++i)
 	{
-		const uint32_t c = e / 64, r = e % 64;
+		const uint32_t c = threadIdx.x / 64 + 4 * i, r = threadIdx.x % 64;
 		across[(c0 + c) * ld_across + r0 + r] = tile[r][c];
 	}
 }
@@ -1033,7 +1106,7 @@ hipError_t pair_launch (tcg_ctx* ctx, const PairArgs& g, uint64_t batch)
 		hipError_t err = hipFuncSetAttribute((const void*) ortho_pair_k<WT,SLABS,MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
 		if (err != hipSuccess) { return err; }
 	}
-	ortho_pair_k<WT,SLABS,MODE><<<(unsigned) (g.tiles * batch), 256, bytes, ctx->stream>>>(g);
+	ortho_pair_k<WT,SLABS,MODE><<<(unsigned) (g.tiles * batch * (MODE == GRAM ? g.parts : 1)), 256, bytes, ctx->stream>>>(g);
 	return hipGetLastError();
 }
 
@@ -1069,15 +1142,36 @@ struct PairCost
 };
 constexpr PairCost pair_costs[4] = {{}, {2, 800, 900, 7000}, {1, 950, 1400, 9000}, {1, 2030, 2600, 16000}};
 
+// Where the tiles of A leave CUs without one, several workgroups share a tile, each a run
+// of its slabs: 12 slabs or more, or bringing the parts together costs more than they save
+// (all five steps, shared and not: 768 x 2048, 3 workgroups a tile, 207 and 227 us; 256 x
+// 4096, 10 a tile, 145 and 220, with runs of 6 slabs 163; 640 x 640, where runs would be of
+// 6 slabs, 147 and 146)
+constexpr uint64_t SHARE_LEAST = 12;
+constexpr double SHARE_ENDS = 7000; // cycles to bring the parts together
+
+/// Workgroups that share a tile of A
+uint32_t gram_parts (const tcg_ctx* ctx, int wt, uint64_t rows, uint64_t slabs, uint64_t batch)
+{
+	if (wt != 1) { return 1; }
+	const uint64_t tm = rows / 64, tiles = tm * (tm + 1) / 2 * batch;
+	uint64_t parts = (uint64_t) ctx->num_cus / tiles;
+	if (parts > slabs / SHARE_LEAST) { parts = slabs / SHARE_LEAST; }
+	if (parts < 2) { return 1; }
+	const uint64_t share = (slabs + parts - 1) / parts;
+	return (uint32_t) ((slabs + share - 1) / share); // none without a slab
+}
+
 /// Cycles of one product with tiles of 64 wt
-double pair_cycles (const tcg_ctx* ctx, int wt, bool symmetric, uint64_t rows_p, uint64_t rows_q, uint64_t slabs, uint64_t batch)
+double pair_cycles (const tcg_ctx* ctx, int wt, bool symmetric, uint64_t rows_p, uint64_t rows_q, uint64_t slabs, uint64_t batch, uint32_t parts = 1)
 {
 	const PairCost& c = pair_costs[wt];
 	const uint64_t tm = (rows_p + 64 * wt - 1) / (64 * wt), tn = (rows_q + 64 * wt - 1) / (64 * wt);
 	const uint64_t tiles = (symmetric ? tm * (tm + 1) / 2 : tm * tn) * batch;
 	const uint64_t room = (uint64_t) ctx->num_cus * c.per_cu;
 	double slab = symmetric ? c.slab : c.apply;
-	if (wt == 1 && tiles <= (uint64_t) ctx->num_cus) { slab = symmetric ? 500 : 650; }
+	if (wt == 1 && tiles * parts <= (uint64_t) ctx->num_cus) { slab = symmetric ? 500 : 650; }
+	if (parts > 1) { return (double) ((slabs + parts - 1) / parts) * slab + c.ends + SHARE_ENDS; }
 	return (double) ((tiles + room - 1) / room) * ((double) slabs * slab + c.ends);
 }
 
@@ -1168,17 +1262,34 @@ int ortho_float (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, u
 	const uint64_t mp = padded(m, 64), np = padded(n, 64);
 	TCG_REQUIRE(ctx, mp / 64 * (np / 64) * batch < (1ull << 31), "tcg_orthogonalize: %llu matrices of %llu x %llu are too many",
 		(unsigned long long) batch, (unsigned long long) rows, (unsigned long long) cols);
+	// A in fp32 goes from GRAM to FACTOR in the order of their tiles: one size for both
+	int wt_gram = 1, wt_apply = 1;
+	double least_gram = 1e300, least_apply = 1e300;
+	for (int wt = 1; wt <= 3; ++wt)
+	{
+		const double both = pair_cycles(ctx, wt, true, mp, mp, np / 32, batch, gram_parts(ctx, wt, mp, np / 32, batch)) + pair_cycles(ctx, wt, true, mp, mp, mp / 32, batch);
+		const double apply = pair_cycles(ctx, wt, false, mp, np, mp / 32, batch);
+		if (both < least_gram) { least_gram = both; wt_gram = wt; }
+		if (apply < least_apply) { least_apply = apply; wt_apply = wt; }
+	}
+	const uint32_t gram_shares = gram_parts(ctx, wt_gram, mp, np / 32, batch);
+	const uint64_t gram_tiles = gram_shares > 1 ? mp / 64 * (mp / 64 + 1) / 2 : 0;
+
 	// X, X^T and X in fp32 before and after a step, A, A in fp32, B; 32 bits an element each
 	const size_t xs = (size_t) mp * np * 2, as = (size_t) mp * mp * 2; // halves
 	const uint32_t parts = norm_parts(rows);
 	const size_t sums_bytes = ((size_t) batch * parts * sizeof(double) + 255) / 256 * 256;
-	const size_t bytes = sums_bytes + (6 * xs + 3 * as) * batch * sizeof(f16);
+	const size_t arrived_bytes = ((size_t) batch * gram_tiles * sizeof(uint32_t) + 255) / 256 * 256;
+	const size_t partial_bytes = (size_t) batch * gram_tiles * gram_shares * 64 * 64 * sizeof(float);
+	const size_t bytes = sums_bytes + arrived_bytes + partial_bytes + (6 * xs + 3 * as) * batch * sizeof(f16);
 	void* mem = nullptr;
 	int rc = tcg_alloc(ctx, bytes, &mem);
 	if (rc != TCG_OK) { return rc; }
 	f16* x[2], *xt[2];
 	float* x32[2];
-	f16* p = reinterpret_cast<f16*>((char*) mem + sums_bytes);
+	uint32_t* arrived = reinterpret_cast<uint32_t*>((char*) mem + sums_bytes);
+	float* partial = reinterpret_cast<float*>((char*) arrived + arrived_bytes);
+	f16* p = reinterpret_cast<f16*>((char*) partial + partial_bytes);
 	for (int k = 0; k < 2; ++k)
 	{
 		x[k] = p; p += xs * batch;
@@ -1194,6 +1305,7 @@ int ortho_float (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, u
 	prep.rows = rows; prep.cols = cols;
 	prep.parts = parts; prep.sums = (double*) mem; prep.eps = eps;
 	prep.scale = scale_of(plan.x[0]);
+	prep.arrived = arrived; prep.arrivals = (uint32_t) gram_tiles;
 	prep.x = x[0]; prep.xt = xt[0]; prep.x32 = x32[0];
 	prep.ldx = np * 2; prep.ldxt = mp * 2;
 	prep.stride_x = prep.stride_xt = xs;
@@ -1202,16 +1314,6 @@ int ortho_float (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, u
 	const uint32_t tiles_x = (uint32_t) ((tall ? mp : np) / 64);
 	ortho_split_k<<<dim3((unsigned) (mp / 64 * (np / 64)), (unsigned) batch), 256, 0, ctx->stream>>>(prep, tiles_x);
 
-	// A in fp32 goes from GRAM to FACTOR in the order of their tiles: one size for both
-	int wt_gram = 1, wt_apply = 1;
-	double least_gram = 1e300, least_apply = 1e300;
-	for (int wt = 1; wt <= 3; ++wt)
-	{
-		const double both = pair_cycles(ctx, wt, true, mp, mp, np / 32, batch) + pair_cycles(ctx, wt, true, mp, mp, mp / 32, batch);
-		const double apply = pair_cycles(ctx, wt, false, mp, np, mp / 32, batch);
-		if (both < least_gram) { least_gram = both; wt_gram = wt; }
-		if (apply < least_apply) { least_apply = apply; wt_apply = wt; }
-	}
 	hipError_t err = hipGetLastError();
 	auto launch = [&] (Product mode, PairArgs& g)
 	{
@@ -1227,6 +1329,8 @@ int ortho_float (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, u
 		g.p = g.q = x[now];
 		g.ldp = g.ldq = np * 2; g.stride_p = g.stride_q = xs;
 		g.slabs = (uint32_t) (np / 32);
+		g.parts = gram_shares; g.share = (g.slabs + g.parts - 1) / g.parts;
+		g.partial = partial; g.arrived = arrived;
 		g.alpha = sa / sx / sx;
 		g.out32 = gram32; g.stride32 = as / 2;
 		g.out = g.out_t = gram;

@@ -129,6 +129,51 @@ def test_several_matrices(ctx, batch, rows, cols, t):
     np.testing.assert_array_equal(got, again)
 
 
+# 3, 8, 24, 2 and 5 workgroups to a tile of A on 256 CUs, mostly with a shorter last run of slabs
+SHARED = [(1, 700, 2000), (1, 260, 3100), (1, 40, 9900), (3, 1000, 330), (2, 190, 2101)]
+
+
+@pytest.mark.parametrize("batch,rows,cols", SHARED)
+def test_tiles_that_workgroups_share(ctx, batch, rows, cols):
+    g = gradient(rows, cols, batch=batch, seed=rows)
+    got = run(ctx, g, pad=1, gap=3)
+    for z in range(batch):
+        close(got[z], g[z])
+    for _ in range(10):  # whoever arrives last, the sums are the same
+        np.testing.assert_array_equal(got, run(ctx, g, pad=1, gap=3))
+
+
+def test_shared_tiles_recorded_and_beside_a_fork(ctx):
+    g, h = gradient(260, 3100, seed=1), gradient(260, 3100, seed=2)
+    wants = [run(ctx, v)[0].reshape(-1) for v in (g, h)]
+    srcs = [ctx.upload(v) for v in (g, h)]
+    dsts = [ctx.upload(np.zeros_like(v)) for v in (g, h)]
+
+    def both():
+        ctx.fork()
+        ctx.orthogonalize(2, 260, 3100, 1, srcs[0].ptr, 3100, 0, dsts[0].ptr, 3100, 0)
+        ctx.fork_end()
+        ctx.orthogonalize(2, 260, 3100, 1, srcs[1].ptr, 3100, 0, dsts[1].ptr, 3100, 0)
+        ctx.join()
+
+    def check():
+        for dst, want in zip(dsts, wants):
+            np.testing.assert_array_equal(dst.get(), want)
+            ctx.fill_zero(dst.ptr, dst.nbytes)
+
+    both()
+    check()
+    ctx.capture_begin()
+    both()
+    graph = ctx.capture_end()
+    for _ in range(3):
+        ctx.graph_launch(graph)
+        check()
+        both()
+        check()
+    ctx.graph_destroy(graph)
+
+
 @pytest.mark.parametrize("rows,cols", [(2000, 2050), (2100, 1900)])
 def test_a_large_matrix(ctx, rows, cols):
     """Enough tiles of 128 x 128 for the chip; singular values of every size, the weakest near zero."""
