@@ -43,13 +43,15 @@ template <> struct AnyVec<double> { using type = f64x2_any; };
 template <typename T>
 constexpr int VN = Vec16<T>::N;
 
-template <typename T, bool RAGGED>
+// ONCE: with the hint that nothing reads or writes this memory again soon
+template <typename T, bool RAGGED, bool ONCE = false>
 __device__ __forceinline__ typename Vec16<T>::type load_vec (const T* row, uint32_t col, uint32_t cols)
 {
 	typename Vec16<T>::type v = {};
 	if (col + VN<T> <= cols)
 	{
-		v = *reinterpret_cast<const typename AnyVec<T>::type*>(row + col);
+		const auto* from = reinterpret_cast<const typename AnyVec<T>::type*>(row + col);
+		v = ONCE ? __builtin_nontemporal_load(from) : *from;
 	}
 	else if constexpr (RAGGED)
 	{
@@ -62,12 +64,14 @@ __device__ __forceinline__ typename Vec16<T>::type load_vec (const T* row, uint3
 	return v;
 }
 
-template <typename T, bool RAGGED>
+template <typename T, bool RAGGED, bool ONCE = false>
 __device__ __forceinline__ void store_vec (T* row, uint32_t col, uint32_t cols, typename Vec16<T>::type v)
 {
 	if (col + VN<T> <= cols)
 	{
-		*reinterpret_cast<typename AnyVec<T>::type*>(row + col) = v;
+		auto* to = reinterpret_cast<typename AnyVec<T>::type*>(row + col);
+		if constexpr (ONCE) { __builtin_nontemporal_store((typename AnyVec<T>::type) v, to); }
+		else { *to = v; }
 	}
 	else if constexpr (RAGGED)
 	{
@@ -265,9 +269,10 @@ struct GradArgs
 	T eps, inv_n;
 };
 
+// ONCE: x, dy and dx are more than the caches hold.
 // (The next row's loads ahead of the row in hand changed nothing: 32768 x 4096 295 us
 // without them, 289 and 301 with them, depending on where the statistics were loaded.)
-template <typename T, int SPAN, int PER, bool RAGGED, bool DX, bool PARAMS>
+template <typename T, int SPAN, int PER, bool RAGGED, bool DX, bool PARAMS, bool ONCE>
 __global__ __launch_bounds__(group_size(SPAN)) void layer_norm_grad_k (GradArgs<T> a)
 {
 	using V = typename Vec16<T>::type;
@@ -293,8 +298,8 @@ __global__ __launch_bounds__(group_size(SPAN)) void layer_norm_grad_k (GradArgs<
 #pragma unroll
 		for (int j = 0; j < PER; ++j)
 		{
-			h[j] = load_vec<T,RAGGED>(x, (j * SPAN + lane) * VN<T>, a.cols);
-			g[j] = load_vec<T,RAGGED>(dy, (j * SPAN + lane) * VN<T>, a.cols);
+			h[j] = load_vec<T,RAGGED,ONCE>(x, (j * SPAN + lane) * VN<T>, a.cols);
+			g[j] = load_vec<T,RAGGED,ONCE>(dy, (j * SPAN + lane) * VN<T>, a.cols);
 		}
 		T m, c = 0, r;
 		if (a.mean)
@@ -338,7 +343,7 @@ __global__ __launch_bounds__(group_size(SPAN)) void layer_norm_grad_k (GradArgs<
 				V out;
 #pragma unroll
 				for (int i = 0; i < VN<T>; ++i) { out[i] = r * (g[j][i] - sg - h[j][i] * sh); }
-				store_vec<T,RAGGED>(dx, (j * SPAN + lane) * VN<T>, a.cols, out);
+				store_vec<T,RAGGED,ONCE>(dx, (j * SPAN + lane) * VN<T>, a.cols, out);
 			}
 		}
 	}
@@ -719,13 +724,25 @@ void norm_launch_per (tcg_ctx* ctx, const NormArgs<T>& a, int per)
 	}
 }
 
+template <typename T, int SPAN, int PER, bool RAGGED, bool ONCE>
+void grad_launch_once (tcg_ctx* ctx, const GradArgs<T>& a, unsigned grid)
+{
+	constexpr unsigned threads = group_size(SPAN);
+	if (a.dx && a.partial) { layer_norm_grad_k<T,SPAN,PER,RAGGED,true,true,ONCE><<<grid, threads, 0, ctx->stream>>>(a); }
+	else if (a.dx) { layer_norm_grad_k<T,SPAN,PER,RAGGED,true,false,ONCE><<<grid, threads, 0, ctx->stream>>>(a); }
+	else { layer_norm_grad_k<T,SPAN,PER,RAGGED,false,true,ONCE><<<grid, threads, 0, ctx->stream>>>(a); }
+}
+
+// 32768 x 4096 (1.6 GB): 264 us with the hint for memory used once, 293 without; 16384 x 2048
+// (400 MB): 69 and 75; 16384 x 1024 (200 MB, in the caches at the next call): 38 and 35.5.
+// Forward it costs as much as it gives (4096 x 16384 126 and 117, 32768 x 4096 180 and 187).
+constexpr uint64_t CACHES = 256ull << 20;
+
 template <typename T, int SPAN, int PER, bool RAGGED>
 void grad_launch (tcg_ctx* ctx, const GradArgs<T>& a, unsigned grid)
 {
-	constexpr unsigned threads = group_size(SPAN);
-	if (a.dx && a.partial) { layer_norm_grad_k<T,SPAN,PER,RAGGED,true,true><<<grid, threads, 0, ctx->stream>>>(a); }
-	else if (a.dx) { layer_norm_grad_k<T,SPAN,PER,RAGGED,true,false><<<grid, threads, 0, ctx->stream>>>(a); }
-	else { layer_norm_grad_k<T,SPAN,PER,RAGGED,false,true><<<grid, threads, 0, ctx->stream>>>(a); }
+	if ((a.dx ? 3 : 2) * a.rows * a.cols * sizeof(T) > CACHES) { grad_launch_once<T,SPAN,PER,RAGGED,true>(ctx, a, grid); }
+	else { grad_launch_once<T,SPAN,PER,RAGGED,false>(ctx, a, grid); }
 }
 
 template <typename T, int SPAN>

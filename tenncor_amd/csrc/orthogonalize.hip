@@ -144,7 +144,7 @@ __device__ __forceinline__ uint64_t place32 (uint32_t rows, uint32_t bi, uint32_
 
 /// A thread's 16 values of the 64 x 64 tile of G at (r0, c0): rows threadIdx.x / 64 + 4 i of
 /// column threadIdx.x % 64, zero outside of G.  No branch around a load, so that all are on
-/// their way together (a branch each, waited for in turn: 13 us instead of 6 us at 768 x 2048)
+/// their way together (a branch each, waited for in turn: 13 us instead of 10 at 768 x 2048)
 template <typename T>
 __device__ __forceinline__ void tile_values (T (&v)[16], const PrepArgs<T>& a, const T* g, uint64_t r0, uint64_t c0)
 {

@@ -176,6 +176,17 @@ def test_sums_over_many_rows(ctx, rows, cols):
             assert other == k or not alone[other].any(), "wrote a gradient that was not wanted"
 
 
+@pytest.mark.parametrize("rows,cols,t", [(400000, 60, np.float32), (70000, 331, np.float32), (6000, 4099, np.float32), (9000, 1300, np.float64)])
+def test_more_than_the_caches_hold(ctx, rows, cols, t):
+    """Rows of every shape of the kernels, with 280 MB of x, g and dx.  The longest chain of a sum over rows: 49."""
+    x, w, b, g = data(rows, cols, t, 6)
+    want = reference(x, w, b, 1e-5, g)
+    got = run_backward(ctx, g, x, w, 1e-5, pad=1)
+    close(got["dx"], want["dx"], want["dx_size"], 300, t)
+    close(got["dw"], want["dw"], want["dw_size"], 300, t)
+    close(got["db"], want["db"], want["db_size"], 150, t)
+
+
 @pytest.mark.parametrize("t", [np.float32, np.float64])
 @pytest.mark.parametrize("cols", [5, 300, 5000, 40000])
 def test_rows_far_from_zero(ctx, cols, t):
