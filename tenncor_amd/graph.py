@@ -545,6 +545,8 @@ class Api:
         """`x` normalised over its dims 0 .. ndims - 1, times weight plus bias (of
         those dims' shape; without: ones and zeros).  One node; its gradients are
         one for x, one for the weight and a REDUCE_SUM for the bias."""
+        if not 1 <= ndims <= 7:
+            raise ValueError("cannot normalise over %d dims: 1 to 7 are possible" % ndims)
         args = [x] + ([weight] if weight is not None else [])
         if bias is not None and weight is not None:
             args.append(bias)

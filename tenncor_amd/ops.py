@@ -140,8 +140,13 @@ def layer_norm(x, weight=None, bias=None, ndims=1, epsilon=1e-5, stats=False):
 def layer_norm_grad(up, x, weight=None, ndims=1, epsilon=1e-5, mean=None, rstd=None):
     """(dx, dweight, dbias) for the gradient `up` that arrives at layer_norm(x, ...)."""
     _same_shape("LAYER_NORM_DX", [up, x])
+    if up.dtype != x.dtype:
+        raise ValueError("the gradient and the tensor are of one type")
     _norm_weight(x, ndims, weight)
     rows, cols = _norm_rows(x, ndims)
+    for kept in (mean, rstd):
+        if kept is not None and (kept.dtype != x.dtype or kept.n != rows):
+            raise ValueError("mean and rstd hold one element of the tensor's type for every row")
     dx = _new(x.ctx, x.shape, x)
     dweight, dbias = (_new(x.ctx, x.shape[:ndims], x) for _ in range(2))
     x.ctx.layer_norm_grad(x.dtype, rows, cols, up.ptr, cols, x.ptr, cols, weight and weight.ptr, epsilon,

@@ -151,3 +151,15 @@ def test_ops_check_their_arguments():
             ops.layer_norm(x, ndims=ndims)
     with pytest.raises(ValueError, match="incompatible shapes"):
         ops.layer_norm_grad(_Fake([4, 2]), x)
+    with pytest.raises(ValueError, match="of one type"):
+        ops.layer_norm_grad(_Fake([4, 3], 1), x)
+    kept = _Fake([1, 3])
+    for mean, rstd in ((_Fake([1, 2]), kept), (kept, _Fake([4, 3])), (_Fake([1, 3], 1), kept), (kept, _Fake([1, 3], 1))):
+        with pytest.raises(ValueError, match="for every row"):
+            ops.layer_norm_grad(x, x, mean=mean, rstd=rstd)
+
+
+def test_more_dims_than_there_are(g, api):
+    for ndims in (0, 8, 257):
+        with pytest.raises(ValueError, match="over %d dims" % ndims):
+            api.layer_norm(var(g, [4, 3]), ndims=ndims)

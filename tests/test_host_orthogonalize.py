@@ -62,3 +62,10 @@ def test_the_update_rule_is_a_graph_like_the_others(g, api):
     assert text.count("(ORTHOGONALIZE") == 1 and "(ASSIGN<" in text or "(ASSIGN" in text
     with pytest.raises(ValueError, match="matrices"):
         graph.Approx(api).muon(loss, [var(g, [3, 4, 2])])
+
+
+def test_three_coefficients():
+    from tenncor_amd import capi
+    for coef in ((1.5, -0.5), (1, 2, 3, 4)):
+        with pytest.raises(ValueError, match="not %d of them" % len(coef)):
+            capi.Context.orthogonalize(None, 2, 1, 1, 1, 0, 1, 1, 0, 1, 1, coef=coef)
