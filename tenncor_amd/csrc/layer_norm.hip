@@ -820,7 +820,7 @@ int grad_chunked (tcg_ctx* ctx, const GradArgs<T>& g, uint64_t cols, double eps,
 	uint32_t parts = 0;
 	if (dweight || dbias)
 	{
-		parts = (uint32_t) (a.rows < 16 ? a.rows : 16);
+		parts = (uint32_t) (a.rows < 16 ? a.rows : a.rows < 16 * 64 ? 16 : a.rows < 128 * 64 ? a.rows / 64 : 128);
 		partial_bytes = (size_t) parts * 2 * cols * sizeof(T);
 	}
 	void* mem = nullptr;

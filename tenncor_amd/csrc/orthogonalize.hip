@@ -63,7 +63,8 @@ __device__ __forceinline__ uint32_t packed (Split s)
 
 // ---- the norm, and the first split -------------------------------------------------
 
-constexpr uint32_t NORM_PARTS = 256; // workgroups that sum one matrix at most
+constexpr uint32_t NORM_PARTS = 512; // workgroups that sum one matrix at most
+constexpr uint64_t NORM_RUN = 1024;  // elements of a row a wave takes at a time
 
 template <typename T>
 struct PrepArgs
@@ -106,13 +107,15 @@ __global__ __launch_bounds__(256) void ortho_norm_k (PrepArgs<T> a)
 	__shared__ double red[4];
 	const T* g = a.g + blockIdx.y * a.stride_g;
 	double sum = 0;
-	// rows dealt to the workgroups' waves, lanes along a row
+	// runs of the rows dealt to the workgroups' waves, lanes along a run
 	const uint32_t wave = threadIdx.x / TCG_WAVE, lane = threadIdx.x & (TCG_WAVE - 1);
-	for (uint64_t row = (uint64_t) blockIdx.x * 4 + wave; row < a.rows; row += (uint64_t) a.parts * 4)
+	const uint64_t runs = (a.cols + NORM_RUN - 1) / NORM_RUN;
+	for (uint64_t at = (uint64_t) blockIdx.x * 4 + wave; at < a.rows * runs; at += (uint64_t) a.parts * 4)
 	{
-		const T* p = g + row * a.ldg;
-#pragma unroll 4
-		for (uint64_t col = lane; col < a.cols; col += TCG_WAVE)
+		const T* p = g + at / runs * a.ldg;
+		const uint64_t from = at % runs * NORM_RUN, to = from + NORM_RUN < a.cols ? from + NORM_RUN : a.cols;
+#pragma unroll 8
+		for (uint64_t col = from + lane; col < to; col += TCG_WAVE)
 		{
 			const double v = p[col];
 			sum += v * v;
@@ -1090,9 +1093,9 @@ uint32_t sum_cut (uint32_t slabs)
 
 uint64_t padded (uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
-uint32_t norm_parts (uint64_t rows)
+uint32_t norm_parts (uint64_t rows, uint64_t cols)
 {
-	const uint64_t want = (rows + 3) / 4;
+	const uint64_t want = (rows * ((cols + NORM_RUN - 1) / NORM_RUN) + 3) / 4;
 	return (uint32_t) (want < NORM_PARTS ? want : NORM_PARTS);
 }
 
@@ -1277,7 +1280,7 @@ int ortho_float (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, u
 
 	// X, X^T and X in fp32 before and after a step, A, A in fp32, B; 32 bits an element each
 	const size_t xs = (size_t) mp * np * 2, as = (size_t) mp * mp * 2; // halves
-	const uint32_t parts = norm_parts(rows);
+	const uint32_t parts = norm_parts(rows, cols);
 	const size_t sums_bytes = ((size_t) batch * parts * sizeof(double) + 255) / 256 * 256;
 	const size_t arrived_bytes = ((size_t) batch * gram_tiles * sizeof(uint32_t) + 255) / 256 * 256;
 	const size_t partial_bytes = (size_t) batch * gram_tiles * gram_shares * 64 * 64 * sizeof(float);
@@ -1386,7 +1389,7 @@ int ortho_double (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, 
 	const uint64_t m = tall ? cols : rows, n = tall ? rows : cols;
 	const uint64_t mp = padded(m, 64), np = padded(n, 64);
 	const size_t xs = (size_t) mp * np, as = (size_t) mp * mp;
-	const uint32_t parts = norm_parts(rows);
+	const uint32_t parts = norm_parts(rows, cols);
 	const size_t sums_bytes = ((size_t) batch * parts * sizeof(double) + 255) / 256 * 256;
 	const size_t bytes = sums_bytes + (4 * xs + 2 * as) * batch * sizeof(double);
 	TCG_REQUIRE(ctx, mp / 16 * (np / 16) * batch < (1ull << 31), "tcg_orthogonalize: %llu matrices of %llu x %llu are too many",
