@@ -469,6 +469,7 @@ __global__ __launch_bounds__(256) void ortho_pair_k (PairArgs g)
 			if (*count + 1 != g.parts) { return; }
 			if (threadIdx.x == 0) { __hip_atomic_store(g.arrived + at, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 			f32x16 all = {};
+#pragma unroll 4
 			for (uint32_t q = 0; q < g.parts; ++q)
 			{
 #pragma unroll
@@ -1147,9 +1148,10 @@ constexpr PairCost pair_costs[4] = {{}, {2, 800, 900, 7000}, {1, 950, 1400, 9000
 
 // Where the tiles of A leave CUs without one, several workgroups share a tile, each a run
 // of its slabs: 12 slabs or more, or bringing the parts together costs more than they save
-// (all five steps, shared and not: 768 x 2048, 3 workgroups a tile, 207 and 227 us; 256 x
-// 4096, 10 a tile, 145 and 220, with runs of 6 slabs 163; 640 x 640, where runs would be of
-// 6 slabs, 147 and 146)
+// (all five steps, shared and not: 768 x 2048, 3 workgroups a tile, 199 and 227 us; 256 x
+// 4096, 10 a tile, 137 and 220, with runs of 6 slabs 20 more; 640 x 640, where runs would
+// be of 6 slabs, 147 and 146).  A part costs the last workgroup about as much as a slab, so
+// no more of them than the root of the slabs (4 x 100000: 290 us with 56 parts, 458 with 256)
 constexpr uint64_t SHARE_LEAST = 12;
 constexpr double SHARE_ENDS = 7000; // cycles to bring the parts together
 
@@ -1160,6 +1162,8 @@ uint32_t gram_parts (const tcg_ctx* ctx, int wt, uint64_t rows, uint64_t slabs, 
 	const uint64_t tm = rows / 64, tiles = tm * (tm + 1) / 2 * batch;
 	uint64_t parts = (uint64_t) ctx->num_cus / tiles;
 	if (parts > slabs / SHARE_LEAST) { parts = slabs / SHARE_LEAST; }
+	const uint64_t most = (uint64_t) ::sqrt((double) slabs);
+	if (parts > most) { parts = most; }
 	if (parts < 2) { return 1; }
 	const uint64_t share = (slabs + parts - 1) / parts;
 	return (uint32_t) ((slabs + share - 1) / share); // none without a slab

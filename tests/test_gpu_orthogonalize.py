@@ -129,7 +129,7 @@ def test_several_matrices(ctx, batch, rows, cols, t):
     np.testing.assert_array_equal(got, again)
 
 
-# 3, 8, 24, 2 and 5 workgroups to a tile of A on 256 CUs, mostly with a shorter last run of slabs
+# 3, 8, 17, 2 and 5 workgroups to a tile of A on 256 CUs, mostly with a shorter last run of slabs
 SHARED = [(1, 700, 2000), (1, 260, 3100), (1, 40, 9900), (3, 1000, 330), (2, 190, 2101)]
 
 
