@@ -22,7 +22,9 @@
 //
 // The sums over rows stay in registers of the waves that walk them, one partial
 // row of dw and db per workgroup goes to memory, and a second launch adds these
-// up in a fixed order: no atomics, the same bits at every call.
+// up in a fixed order: no atomics, the same bits at every call.  All gradients of a
+// few rows with known statistics take one launch, in which workgroups of their own
+// sum over the rows.
 #include "tcg_internal.hpp"
 
 #include <limits>
@@ -273,7 +275,7 @@ struct GradArgs
 // (The next row's loads ahead of the row in hand changed nothing: 32768 x 4096 295 us
 // without them, 289 and 301 with them, depending on where the statistics were loaded.)
 template <typename T, int SPAN, int PER, bool RAGGED, bool DX, bool PARAMS, bool ONCE>
-__global__ __launch_bounds__(group_size(SPAN)) void layer_norm_grad_k (GradArgs<T> a)
+__device__ __forceinline__ void grad_rows (const GradArgs<T>& a, uint32_t group, uint32_t groups)
 {
 	using V = typename Vec16<T>::type;
 	__shared__ T red[4 * group_size(SPAN) / TCG_WAVE];
@@ -289,8 +291,8 @@ __global__ __launch_bounds__(group_size(SPAN)) void layer_norm_grad_k (GradArgs<
 		w[j] = V{} + (T) 1;
 		if (DX && a.weight) { w[j] = load_vec<T,RAGGED>(a.weight, (j * SPAN + lane) * VN<T>, a.cols); }
 	}
-	const uint64_t step = (uint64_t) gridDim.x * ROWS;
-	for (uint64_t row = (uint64_t) blockIdx.x * ROWS + threadIdx.x / SPAN; row < a.rows; row += step)
+	const uint64_t step = (uint64_t) groups * ROWS;
+	for (uint64_t row = (uint64_t) group * ROWS + threadIdx.x / SPAN; row < a.rows; row += step)
 	{
 		const T* x = a.x + row * a.ldx;
 		const T* dy = a.dy + row * a.lddy;
@@ -349,7 +351,7 @@ __global__ __launch_bounds__(group_size(SPAN)) void layer_norm_grad_k (GradArgs<
 	}
 	if constexpr (PARAMS)
 	{
-		T* out = a.partial + (uint64_t) blockIdx.x * 2 * a.cols;
+		T* out = a.partial + (uint64_t) group * 2 * a.cols;
 		if constexpr (ROWS > 1)
 		{
 			// the row slots of the workgroup hold sums of the same columns: added in their order
@@ -382,6 +384,80 @@ __global__ __launch_bounds__(group_size(SPAN)) void layer_norm_grad_k (GradArgs<
 			store_vec<T,RAGGED>(out + a.cols, (j * SPAN + lane) * VN<T>, a.cols, db[j]);
 		}
 	}
+}
+
+template <typename T, int SPAN, int PER, bool RAGGED, bool DX, bool PARAMS, bool ONCE>
+__global__ __launch_bounds__(group_size(SPAN)) void layer_norm_grad_k (GradArgs<T> a)
+{
+	grad_rows<T,SPAN,PER,RAGGED,DX,PARAMS,ONCE>(a, blockIdx.x, gridDim.x);
+}
+
+// dw and db of the four vectors of columns of a strip, straight from x and dy: 64 lanes take
+// every 64th row each and are added up in the order of their lanes' tree and waves
+template <typename T>
+__device__ __forceinline__ void grad_strip (const GradArgs<T>& a, uint32_t strip, T* dweight, T* dbias)
+{
+	using V = typename Vec16<T>::type;
+	__shared__ V meet[2][4][4];
+	const uint32_t place = threadIdx.x % 4, lane = threadIdx.x % TCG_WAVE, wave = threadIdx.x / TCG_WAVE;
+	const uint32_t col = (strip * 4 + place) * VN<T>;
+	// the row's last whole vector for lanes that would read past it; they keep what is their own
+	const uint32_t from = col + VN<T> <= a.cols ? col : a.cols - VN<T>;
+	V dw = {}, db = {};
+#pragma unroll 4
+	for (uint64_t row = threadIdx.x / 4; row < a.rows; row += 64)
+	{
+		const V x = *reinterpret_cast<const typename AnyVec<T>::type*>(a.x + row * a.ldx + from);
+		const V g = *reinterpret_cast<const typename AnyVec<T>::type*>(a.dy + row * a.lddy + from);
+		const T m = a.mean[row], r = a.rstd[row];
+#pragma unroll
+		for (int i = 0; i < VN<T>; ++i)
+		{
+			dw[i] += g[i] * ((x[i] - m) * r);
+			db[i] += g[i];
+		}
+	}
+#pragma unroll
+	for (int d = 4; d < TCG_WAVE; d *= 2)
+	{
+#pragma unroll
+		for (int i = 0; i < VN<T>; ++i)
+		{
+			dw[i] += __shfl_xor(dw[i], d);
+			db[i] += __shfl_xor(db[i], d);
+		}
+	}
+	if (lane < 4)
+	{
+		meet[0][wave][place] = dw;
+		meet[1][wave][place] = db;
+	}
+	__syncthreads();
+	if (threadIdx.x >= 4) { return; }
+	for (int k = 1; k < 4; ++k)
+	{
+		dw += meet[0][k][place];
+		db += meet[1][k][place];
+	}
+#pragma unroll
+	for (int i = 0; i < VN<T>; ++i)
+	{
+		if (from + i >= col && from + i < a.cols)
+		{
+			if (dweight) { dweight[from + i] = dw[i]; }
+			if (dbias) { dbias[from + i] = db[i]; }
+		}
+	}
+}
+
+// All three gradients of a few rows with known statistics in one launch: the first
+// `strips` workgroups take dw and db, the others dx.  x and dy are read twice, which
+// costs less than a second launch as long as they are small.
+template <typename T, int SPAN, int PER, bool RAGGED>
+__global__ __launch_bounds__(256) void layer_norm_grad_few_k (GradArgs<T> a, uint32_t strips, T* dweight, T* dbias)
+{
+	if (blockIdx.x < strips) { grad_strip(a, blockIdx.x, dweight, dbias); }
+	else { grad_rows<T,SPAN,PER,RAGGED,true,false,false>(a, blockIdx.x - strips, gridDim.x - strips); }
 }
 
 // dw[col], db[col] = the sums over `parts` partial rows, 32 columns a workgroup,
@@ -764,6 +840,26 @@ void grad_launch_per (tcg_ctx* ctx, const GradArgs<T>& a, int per, unsigned grid
 	}
 }
 
+template <typename T, int SPAN, int PER>
+void grad_few_launch (tcg_ctx* ctx, const GradArgs<T>& a, T* dweight, T* dbias)
+{
+	const unsigned strips = (unsigned) ((a.cols + 4 * VN<T> - 1) / (4 * VN<T>));
+	const unsigned grid = strips + (unsigned) ((a.rows + rows_at_once(SPAN) - 1) / rows_at_once(SPAN));
+	if (a.cols % VN<T>) { layer_norm_grad_few_k<T,SPAN,PER,true><<<grid, 256, 0, ctx->stream>>>(a, strips, dweight, dbias); }
+	else { layer_norm_grad_few_k<T,SPAN,PER,false><<<grid, 256, 0, ctx->stream>>>(a, strips, dweight, dbias); }
+}
+
+template <typename T, int SPAN>
+void grad_few_launch_per (tcg_ctx* ctx, const GradArgs<T>& a, int per, T* dweight, T* dbias)
+{
+	switch (per)
+	{
+		case 1: grad_few_launch<T,SPAN,1>(ctx, a, dweight, dbias); break;
+		case 2: grad_few_launch<T,SPAN,2>(ctx, a, dweight, dbias); break;
+		default: grad_few_launch<T,SPAN,4>(ctx, a, dweight, dbias); break;
+	}
+}
+
 /// Grid of a kernel that walks rows x chunks
 unsigned chunk_grid (const tcg_ctx* ctx, uint64_t work)
 {
@@ -883,6 +979,11 @@ int norm_run (tcg_ctx* ctx, uint64_t rows, uint64_t cols, const void* x, uint64_
 	return TCG_OK;
 }
 
+// All gradients in one launch, and in two: 256 x 512 4.6 and 6.7-7.3 us, 512 x 4096 9.6 and
+// 16.7, 768 x 3000 11.4 and 13.3; 1024 x 2048 14.2 and 11.9, 2048 x 512 10.2 and 8.1.  (Rows of
+// 1024 lanes: 200 x 8192 8.7 and 13.1, but 768 x 8192 26 and 20, 500 x 16000 36 and 30.)
+constexpr uint64_t FEW_ROWS = 768;
+
 template <typename T>
 int grad_run (tcg_ctx* ctx, uint64_t rows, uint64_t cols, const void* dy, uint64_t lddy, const void* x, uint64_t ldx,
 	const void* weight, const void* mean, const void* rstd, double eps, void* dx, uint64_t lddx, void* dweight, void* dbias)
@@ -899,6 +1000,19 @@ int grad_run (tcg_ctx* ctx, uint64_t rows, uint64_t cols, const void* dy, uint64
 	a.cols = (uint32_t) cols;
 	a.eps = (T) eps;
 	a.inv_n = (T) (1. / (double) cols);
+	// one launch for a few rows; dx must not lie where dw's sums still read
+	if (dx && (dweight || dbias) && mean && dx != x && dx != dy && cols >= VN<T> && shape.span <= 256 && rows <= FEW_ROWS)
+	{
+		switch (shape.span)
+		{
+			case 16: grad_few_launch<T,16,1>(ctx, a, (T*) dweight, (T*) dbias); break;
+			case 32: grad_few_launch<T,32,1>(ctx, a, (T*) dweight, (T*) dbias); break;
+			case 64: grad_few_launch_per<T,64>(ctx, a, shape.per, (T*) dweight, (T*) dbias); break;
+			default: grad_few_launch_per<T,256>(ctx, a, shape.per, (T*) dweight, (T*) dbias); break;
+		}
+		hipError_t err = hipGetLastError();
+		return err == hipSuccess ? TCG_OK : tcg_fail(ctx, TCG_ERR_HIP, "launch of layer_norm_grad failed: %s", hipGetErrorString(err));
+	}
 	const uint64_t at_once = rows_at_once(shape.span), groups = (rows + at_once - 1) / at_once;
 	const bool params = dweight || dbias;
 	// with the sums over rows every workgroup leaves a partial row behind: no more

@@ -176,6 +176,27 @@ def test_sums_over_many_rows(ctx, rows, cols):
             assert other == k or not alone[other].any(), "wrote a gradient that was not wanted"
 
 
+@pytest.mark.parametrize("t", [np.float32, np.float64])
+@pytest.mark.parametrize("rows", [1, 63, 64, 65, 129, 700, 768, 769, 1500])
+@pytest.mark.parametrize("cols", [1, 3, 4, 30, 64, 130, 515, 1100, 4096, 4100])
+def test_all_gradients_with_known_statistics(ctx, rows, cols, t):
+    """Few rows take one launch for all gradients, more rows two; the same bits at every call."""
+    x, w, b, g = data(rows, cols, t, rows + cols)
+    full = reference(x, w, b, 1e-5)
+    stats = [full["mean"].astype(t), full["rstd"].astype(t)]
+    want = reference(x, w, b, 1e-5, g, *stats)
+    for names in (("dx", "dw", "db"), ("dx", "dw"), ("dx", "db")):
+        got = run_backward(ctx, g, x, w, 1e-5, stats, pad=1, shift=1, want=names)
+        for k, ops in (("dx", 300), ("dw", 300), ("db", 150)):
+            if k in names:
+                close(got[k], want[k], want[k + "_size"], ops, t)
+            else:
+                assert not got[k].any(), "wrote a gradient that was not wanted"
+        again = run_backward(ctx, g, x, w, 1e-5, stats, pad=1, shift=1, want=names)
+        for k in got:
+            np.testing.assert_array_equal(got[k], again[k])
+
+
 @pytest.mark.parametrize("rows,cols,t", [(400000, 60, np.float32), (70000, 331, np.float32), (6000, 4099, np.float32), (9000, 1300, np.float64)])
 def test_more_than_the_caches_hold(ctx, rows, cols, t):
     """Rows of every shape of the kernels, with 280 MB of x, g and dx.  The longest chain of a sum over rows: 49."""
@@ -243,6 +264,24 @@ def test_in_place(ctx, rows, cols):
         np.testing.assert_array_equal(out.get().reshape(rows, cols), grads["dx"])
         np.testing.assert_array_equal(ow.get(), grads["dw"])
         np.testing.assert_array_equal(ob.get(), grads["db"])
+
+
+@pytest.mark.parametrize("rows,cols", [(300, 64), (20, 1500)])
+def test_in_place_with_known_statistics(ctx, rows, cols):
+    """dx over dy or x: the sums over rows have read both before."""
+    t = np.float32
+    x, w, b, g = data(rows, cols, t, 14)
+    full = reference(x, w, b, 1e-5)
+    stats = [full["mean"].astype(t), full["rstd"].astype(t)]
+    want = reference(x, w, b, 1e-5, g, *stats)
+    for where in ("dy", "x"):
+        bx, bg, bw, bm, br, ow, ob = (ctx.upload(v) for v in (x, g, w, *stats, w, w))
+        out = bg if where == "dy" else bx
+        ctx.layer_norm_grad(CODE[t], rows, cols, bg.ptr, cols, bx.ptr, cols, bw.ptr, 1e-5, dx=out.ptr, lddx=cols,
+                            dweight=ow.ptr, dbias=ob.ptr, mean=bm.ptr, rstd=br.ptr)
+        close(out.get().reshape(rows, cols), want["dx"], want["dx_size"], 300, t)
+        close(ow.get(), want["dw"], want["dw_size"], 300, t)
+        close(ob.get(), want["db"], want["db_size"], 150, t)
 
 
 def test_no_rows(ctx):
