@@ -673,7 +673,7 @@ int tcg_layer_norm (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols,
  *   dx      = r (dy weight - mean(dy weight) - h mean(dy weight h))
  *   dweight = sum over rows of dy h      dbias = sum over rows of dy
  * Each of dx, dweight and dbias may be NULL (not all three); what is wanted
- * together is computed in one pass over x and dy.  mean / rstd: what the forward
+ * together costs less than one call each.  mean / rstd: what the forward
  * pass left, or both NULL, and they are taken from x again (eps is used only
  * then).  The sums over rows run in a fixed order: the same bits at every call.
  * dx may be dy or x (same leading dim).  No rows: dweight and dbias are zero. */
