@@ -1056,14 +1056,17 @@ bool follow (Plan& p)
 			factor = std::fmax(factor, std::fabs(q * (p.b + q * p.c)));
 		};
 		at(top * top);
-		if (p.c != 0) { at(-p.b / (2 * p.c)); }
+		at(-p.b / (2 * p.c)); // c = 0: infinite or NaN, neither is in range
 		const double inner = 9 * p.b * p.b - 20 * p.a * p.c;
-		if (p.c != 0 && inner >= 0)
+		if (inner >= 0)
 		{
-			at((-3 * p.b + std::sqrt(inner)) / (10 * p.c));
-			at((-3 * p.b - std::sqrt(inner)) / (10 * p.c));
+			// the roots of 5 c q^2 + 3 b q + a without a difference of neighbouring values: with a c
+			// that is almost zero, as the sum of a caller's roundings, -3 b + sqrt(inner) would be 0
+			// and the polynomial's largest value missed
+			const double w = -(3 * p.b + std::copysign(std::sqrt(inner), p.b)) / 2;
+			at(w / (5 * p.c));
+			at(p.a / w);
 		}
-		else if (p.c == 0 && p.b != 0) { at(-p.a / (3 * p.b)); }
 		if (!(next <= 1e300 && factor <= 1e12)) { return false; }
 		p.gram.push_back(top * top);
 		p.factor.push_back(factor * 1.0001);

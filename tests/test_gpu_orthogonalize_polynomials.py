@@ -1,0 +1,51 @@
+"""tcg_orthogonalize with polynomials other than the usual one: which are taken and
+which refused, and what those come to whose terms lie far apart.
+
+Tolerances: as derived in test_gpu_orthogonalize, tol = eta sum_k D^(steps - 1 - k) |X_k|,
+where eta allows for a B of norm 4 and an a of 4 at most.  A step rounds a X + B X, a
+value of up to (|a| + F_k) |X_k| with F_k the largest norm of B, once and B by 2^-22 of
+its norm: where a or F_k is larger, |X_k| counts max(1, F_k / 4, |a| / 4) times.
+"""
+import numpy as np
+import pytest
+
+from test_gpu_orthogonalize import ctx, eta, gradient, run  # noqa: F401 (ctx is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def close(got, g, steps, coef):
+    a, b, c = coef
+    x = g.astype(np.float64)
+    x = x / (np.linalg.norm(x) + 1e-7)
+    top, slopes, sizes = 1.0, [], []
+    for _ in range(steps):
+        s = np.linspace(0, top, 4001)
+        slopes.append(max(abs(a + 3 * b * s ** 2 + 5 * c * s ** 4).max(), abs(a + b * s ** 2 + c * s ** 4).max(), 1.0))
+        sizes.append(np.linalg.norm(x) * max(1.0, abs(b * s ** 2 + c * s ** 4).max() / 4, abs(a) / 4))
+        top = abs(s * (a + b * s ** 2 + c * s ** 4)).max() * 1.001
+        gram = x @ x.T
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    assert np.isfinite(got).all()
+    tol = eta(g.dtype.type, g.shape) * sum(np.prod(slopes[k + 1:]) * sizes[k] for k in range(steps))
+    off = np.linalg.norm(got.astype(np.float64) - x)
+    assert off <= tol, "%g of the tolerance, %g of the result" % (off / tol, off / np.linalg.norm(x))
+
+
+@pytest.mark.parametrize("rows,cols", [(40, 56), (300, 200)])
+@pytest.mark.parametrize("t", [np.float32, np.float64])
+@pytest.mark.parametrize("a,b", [(2.598, -2.598), (1.5, -0.5)])
+def test_a_last_coefficient_that_is_almost_zero(ctx, rows, cols, t, a, b):
+    """0.1 + 0.2 - 0.3 in place of nothing: the polynomial is largest where it is without that
+    coefficient.  The term itself is below a rounding of every result."""
+    g = gradient(rows, cols, t, seed=21)
+    for c in (5.6e-17, 1e-18, -1e-17, 1e-300):
+        close(run(ctx, g, steps=3, coef=(a, b, c))[0], g[0], 3, (a, b, 0.0))
+
+
+@pytest.mark.parametrize("c", [0.0, 1e-17, -1e-18])
+def test_growth_between_the_ends_is_refused(ctx, c):
+    """p(1) = 0, but 30 s - 30 s^3 is 11.5 at s^2 = 1/3, and 45000 behind that."""
+    from tenncor_amd import capi
+    with pytest.raises(capi.TcgError, match="grow past"):
+        run(ctx, gradient(8, 9), steps=4, coef=(30.0, -30.0, c))
