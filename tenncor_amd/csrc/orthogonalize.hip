@@ -1046,6 +1046,7 @@ bool follow (Plan& p)
 	{
 		if (!(top <= 1e6)) { return false; } // a NaN as well
 		p.x.push_back(top);
+		if (k == p.steps) { break; } // nothing is made of the last X
 		// both are largest at an end or where their slope is zero: with q = s^2,
 		// p' = a + 3 b q + 5 c q^2 and (b q + c q^2)' = b + 2 c q
 		double next = 0, factor = 0;

@@ -49,3 +49,15 @@ def test_growth_between_the_ends_is_refused(ctx, c):
     from tenncor_amd import capi
     with pytest.raises(capi.TcgError, match="grow past"):
         run(ctx, gradient(8, 9), steps=4, coef=(30.0, -30.0, c))
+
+
+@pytest.mark.parametrize("rows,cols", [(40, 56), (300, 200)])
+@pytest.mark.parametrize("t", [np.float32, np.float64])
+@pytest.mark.parametrize("steps,coef,top", [(2, (3.0, 2.0, 1.0), 8240), (1, (1.0, 0.0, 1e4), 10001), (2, (900.0, 0.0, 0.0), 810000)])
+def test_values_below_a_million_after_the_last_step(ctx, rows, cols, t, steps, coef, top):
+    """What another step would make of them does not matter."""
+    from tenncor_amd import capi
+    g = gradient(rows, cols, t, seed=22)
+    close(run(ctx, g, steps=steps, coef=coef)[0], g[0], steps, coef)
+    with pytest.raises(capi.TcgError, match="grow past"):
+        run(ctx, g, steps=steps + 1, coef=coef)
