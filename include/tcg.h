@@ -692,9 +692,13 @@ int tcg_layer_norm_grad (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols,
  * the values towards one the result is near the closest orthogonal matrix.  A
  * matrix of zeros stays one (eps > 0); a NaN or an infinity makes its whole matrix
  * NaN and leaves the others alone.
- * float and double.  In float the products run on half-precision matrix
- * instructions with every operand as two halves (22 bits and more of each value)
- * and sums in fp32: results are as near to the formulas as with fp32 products.
+ * float and double.  In float the products run on half-precision matrix instructions
+ * with every operand as two halves and sums in fp32; a half's value is kept to 2^-22 of
+ * itself or, where it is small, to 2^-39 of the largest value that the iteration can give
+ * for any matrix, and the term coef[0] X is taken from X in fp32.  Five steps with the
+ * usual coefficients are 3e-6 of the result off the formulas.  Where coef[0] is below
+ * 2^-17 of what coef[1] s^2 + coef[2] s^4 can reach, that would not be enough, and the
+ * products are in double.
  * 1 to 64 steps; coefficients under which values of up to one grow past 1e6 are
  * refused.  out may be in, laid out alike.  The reference has no such operator. */
 int tcg_orthogonalize (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols, uint64_t batch,

@@ -24,7 +24,8 @@
 // that are added up apart, so that neither a part nor their sum is a long chain of
 // roundings (sum_cut below).
 //
-// double: the same steps on fp64 matrix instructions (78.6 TFLOP/s).
+// double: the same steps on fp64 matrix instructions (78.6 TFLOP/s); they also take the
+// floats of a polynomial whose terms lie too far apart for halves (halves_hold below).
 #include "tcg_internal.hpp"
 
 #include <cmath>
@@ -78,12 +79,12 @@ struct PrepArgs
 	float scale;
 	uint32_t* arrived; // [batch][arrivals], cleared here for the products that count in them
 	uint32_t arrivals;
-	// float: X and X^T as split matrices, padded; double: dense, padded
+	// products of halves: X and X^T as split matrices, padded; in double: dense, padded
 	f16* x;
 	f16* xt;
 	uint64_t ldx, stride_x, ldxt, stride_xt;
 	float* x32; // X in fp32, place32
-	T* dense[2]; // X, X^T
+	double* dense[2]; // X, X^T
 	uint64_t stride_dense;
 	bool tall; // X = G^T
 };
@@ -863,13 +864,14 @@ struct DoubleArgs
 	double* out;   // (i, j)
 	double* out_t; // (j, i)
 	uint64_t ldo, ldot, stride_o, stride_ot;
-	double* last;
+	void* last; // OUT
 	uint64_t ldl, stride_l;
 	uint32_t m, n;
 	bool tall;
 };
 
-template <int KSPLIT, int TI, int MODE>
+// OUT: the type of the caller's matrix, which LAST writes
+template <int KSPLIT, int TI, int MODE, typename OUT>
 __global__ __launch_bounds__(256) void ortho_double_k (DoubleArgs g)
 {
 	constexpr bool SYMMETRIC = MODE == GRAM || MODE == FACTOR;
@@ -957,6 +959,7 @@ __global__ __launch_bounds__(256) void ortho_double_k (DoubleArgs g)
 	{
 		if (n + u < groups) { multiply(ring[u]); }
 	}
+	OUT* last = static_cast<OUT*>(g.last) + batch * g.stride_l; // NULL and not used but by LAST
 	double* mine = meet + (KSPLIT == 1 ? 0 : wave * TILE * PITCH);
 #pragma unroll
 	for (int i = 0; i < TI; ++i)
@@ -983,7 +986,7 @@ __global__ __launch_bounds__(256) void ortho_double_k (DoubleArgs g)
 		v *= g.alpha;
 		if constexpr (MODE != GRAM) { v += g.beta * add[t]; }
 		if constexpr (MODE != LAST) { g.out[batch * g.stride_o + (uint64_t) (i0 + i) * g.ldo + j0 + j] = v; }
-		else if (!g.tall && i0 + i < g.m && j0 + j < g.n) { g.last[batch * g.stride_l + (uint64_t) (i0 + i) * g.ldl + j0 + j] = v; }
+		else if (!g.tall && i0 + i < g.m && j0 + j < g.n) { last[(uint64_t) (i0 + i) * g.ldl + j0 + j] = (OUT) v; }
 		meet[i * PITCH + j] = v; // read by this lane alone until now
 	}
 	__syncthreads();
@@ -994,18 +997,19 @@ __global__ __launch_bounds__(256) void ortho_double_k (DoubleArgs g)
 		const uint32_t e = t * 256 + threadIdx.x, j = e / TILE, i = e % TILE;
 		const double v = meet[i * PITCH + j];
 		if constexpr (MODE != LAST) { g.out_t[batch * g.stride_ot + (uint64_t) (j0 + j) * g.ldot + i0 + i] = v; }
-		else if (i0 + i < g.m && j0 + j < g.n) { g.last[batch * g.stride_l + (uint64_t) (j0 + j) * g.ldl + i0 + i] = v; }
+		else if (i0 + i < g.m && j0 + j < g.n) { last[(uint64_t) (j0 + j) * g.ldl + i0 + i] = (OUT) v; }
 	}
 }
 
 // X = G / (|G| + eps) and X^T, padded: a 64 x 64 tile a workgroup
-__global__ __launch_bounds__(256) void ortho_scale_k (PrepArgs<double> a, uint32_t tiles_x)
+template <typename T>
+__global__ __launch_bounds__(256) void ortho_scale_k (PrepArgs<T> a, uint32_t tiles_x)
 {
 	__shared__ double red[4];
 	__shared__ double tile[64][65];
 	const uint32_t batch = blockIdx.y;
 	const uint64_t r0 = (uint64_t) (blockIdx.x / tiles_x) * 64, c0 = (uint64_t) (blockIdx.x % tiles_x) * 64;
-	double v[16];
+	T v[16];
 	tile_values(v, a, a.g + batch * a.stride_g, r0, c0);
 	const double inv = inverse_norm(a, batch, red);
 	double* along = a.dense[a.tall] + batch * a.stride_dense;
@@ -1072,6 +1076,22 @@ bool follow (Plan& p)
 		p.gram.push_back(top * top);
 		p.factor.push_back(factor * 1.0001);
 		top = next * 1.0001;
+	}
+	return true;
+}
+
+/// Whether two halves hold enough of a step's operands.  Their scale follows the largest
+/// value that any matrix can have, and what a half loses at the lower end is 2^-39 of
+/// that (2^-25 where the largest lies at 2^14 or more), however small this matrix's own
+/// values are.  Of A and B it is 2^-39 F with F the largest value of B, and next to a X,
+/// which is taken in fp32, no more than 2^-22 of the result if |a| >= 2^-17 F.  A
+/// polynomial without a linear term has no such measure to go by (s^3 in float, 300 x
+/// 200: off by 6.7e-6 after two steps, zeros after three): its products are in double.
+bool halves_hold (const Plan& p)
+{
+	for (double factor : p.factor)
+	{
+		if (std::fabs(p.a) < std::ldexp(factor, -17)) { return false; }
 	}
 	return true;
 }
@@ -1377,21 +1397,23 @@ int ortho_float (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, u
 	return rc;
 }
 
-template <int KSPLIT, int TI>
+template <int KSPLIT, int TI, typename T>
 void double_launch (tcg_ctx* ctx, Product mode, const DoubleArgs& g, uint64_t batch)
 {
 	const unsigned grid = (unsigned) (g.tiles * batch);
 	switch (mode)
 	{
-		case GRAM: ortho_double_k<KSPLIT,TI,GRAM><<<grid, 256, 0, ctx->stream>>>(g); break;
-		case FACTOR: ortho_double_k<KSPLIT,TI,FACTOR><<<grid, 256, 0, ctx->stream>>>(g); break;
-		case APPLY: ortho_double_k<KSPLIT,TI,APPLY><<<grid, 256, 0, ctx->stream>>>(g); break;
-		default: ortho_double_k<KSPLIT,TI,LAST><<<grid, 256, 0, ctx->stream>>>(g); break;
+		case GRAM: ortho_double_k<KSPLIT,TI,GRAM,double><<<grid, 256, 0, ctx->stream>>>(g); break;
+		case FACTOR: ortho_double_k<KSPLIT,TI,FACTOR,double><<<grid, 256, 0, ctx->stream>>>(g); break;
+		case APPLY: ortho_double_k<KSPLIT,TI,APPLY,double><<<grid, 256, 0, ctx->stream>>>(g); break;
+		default: ortho_double_k<KSPLIT,TI,LAST,T><<<grid, 256, 0, ctx->stream>>>(g); break;
 	}
 }
 
-int ortho_double (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, uint64_t batch, const double* in, uint64_t ldg,
-	uint64_t stride_g, double eps, double* out, uint64_t ldo, uint64_t stride_o)
+/// The iteration in double, of matrices of type T
+template <typename T>
+int ortho_double (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, uint64_t batch, const T* in, uint64_t ldg,
+	uint64_t stride_g, double eps, T* out, uint64_t ldo, uint64_t stride_o)
 {
 	const bool tall = rows > cols;
 	const uint64_t m = tall ? cols : rows, n = tall ? rows : cols;
@@ -1410,7 +1432,7 @@ int ortho_double (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, 
 	for (int k = 0; k < 4; ++k, at += xs * batch) { x[k / 2][k % 2] = at; }
 	double* gram = at;
 	double* factor = gram + as * batch;
-	PrepArgs<double> prep = {};
+	PrepArgs<T> prep = {};
 	prep.g = in; prep.ldg = ldg; prep.stride_g = stride_g;
 	prep.rows = rows; prep.cols = cols;
 	prep.parts = parts; prep.sums = (double*) mem; prep.eps = eps;
@@ -1418,8 +1440,8 @@ int ortho_double (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, 
 	prep.stride_dense = xs;
 	prep.ldx = np; prep.ldxt = mp;
 	prep.tall = tall;
-	ortho_norm_k<double><<<dim3(parts, (unsigned) batch), 256, 0, ctx->stream>>>(prep);
-	ortho_scale_k<<<dim3((unsigned) (mp / 64 * (np / 64)), (unsigned) batch), 256, 0, ctx->stream>>>(prep, (uint32_t) ((tall ? mp : np) / 64));
+	ortho_norm_k<T><<<dim3(parts, (unsigned) batch), 256, 0, ctx->stream>>>(prep);
+	ortho_scale_k<T><<<dim3((unsigned) (mp / 64 * (np / 64)), (unsigned) batch), 256, 0, ctx->stream>>>(prep, (uint32_t) ((tall ? mp : np) / 64));
 	// Tiles of 64 where there are two for every CU, of 16 where tiles of 32 would leave half
 	// of the CUs without one (256 x 256: 127 us with tiles of 32, 85 with tiles of 16;
 	// 1024 x 1024: 840 us with tiles of 32, 1000 with tiles of 64, 1460 with tiles of 16)
@@ -1438,9 +1460,9 @@ int ortho_double (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, 
 		g.tiles = (uint32_t) tiles(tile);
 		switch (tile)
 		{
-			case 64: double_launch<1,2>(ctx, mode, g, batch); break;
-			case 32: double_launch<4,2>(ctx, mode, g, batch); break;
-			default: double_launch<4,1>(ctx, mode, g, batch); break;
+			case 64: double_launch<1,2,T>(ctx, mode, g, batch); break;
+			case 32: double_launch<4,2,T>(ctx, mode, g, batch); break;
+			default: double_launch<4,1,T>(ctx, mode, g, batch); break;
 		}
 	};
 	for (int k = 0; k < plan.steps; ++k)
@@ -1523,9 +1545,10 @@ int tcg_orthogonalize (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols, ui
 		TCG_REQUIRE(ctx, follow(plan), "tcg_orthogonalize: with the polynomial %g s + %g s^3 + %g s^5 singular values grow past 1e6",
 			coef[0], coef[1], coef[2]);
 		if (batch == 1) { stride_i = stride_o = 0; }
-		return dtype == TCG_FLOAT ?
+		if (dtype == TCG_DOUBLE) { return ortho_double(ctx, plan, rows, cols, batch, (const double*) in, ldi, stride_i, eps, (double*) out, ldo, stride_o); }
+		return halves_hold(plan) ?
 			ortho_float(ctx, plan, rows, cols, batch, (const float*) in, ldi, stride_i, eps, (float*) out, ldo, stride_o) :
-			ortho_double(ctx, plan, rows, cols, batch, (const double*) in, ldi, stride_i, eps, (double*) out, ldo, stride_o);
+			ortho_double(ctx, plan, rows, cols, batch, (const float*) in, ldi, stride_i, eps, (float*) out, ldo, stride_o);
 	}
 	catch (const std::bad_alloc&)
 	{

@@ -61,3 +61,26 @@ def test_values_below_a_million_after_the_last_step(ctx, rows, cols, t, steps, c
     close(run(ctx, g, steps=steps, coef=coef)[0], g[0], steps, coef)
     with pytest.raises(capi.TcgError, match="grow past"):
         run(ctx, g, steps=steps + 1, coef=coef)
+
+
+# (rows, cols, batch): one workgroup, 64 x 64 tiles wide and tall, several matrices
+@pytest.mark.parametrize("rows,cols,batch", [(1, 1, 1), (40, 56, 1), (300, 200, 1), (200, 310, 2), (5, 700, 3), (513, 777, 1)])
+@pytest.mark.parametrize("steps,coef", [(1, (0.0, 1.0, 0.0)), (2, (0.0, 1.0, 0.0)), (3, (0.0, 1.0, 0.0)), (2, (0.0, 0.0, 1.0)),
+                                        (3, (1e-7, 1.0, 0.5)), (2, (1e-6, -1.0, 2.0))])
+def test_without_a_linear_term_worth_the_name(ctx, rows, cols, batch, steps, coef):
+    """s -> s^3 three times is s^27: results far below the largest that any matrix could
+    give.  Products in 64 bits, one rounding to float: 2^-24 of each element; in the norm
+    2^-24 of the result's, and as much again for what the roundings in 64 bits come to
+    (at most (8 + 777) sqrt(777) 2^-53 a step, taken up to 5 x 5 x 5 times by the steps:
+    2^-31), and half of the smallest float an element."""
+    g = gradient(rows, cols, batch=batch, seed=23)
+    for pad, gap, shift, in_place in ((0, 0, 0, False), (3, 5, 1, True)):
+        got = run(ctx, g, pad=pad, gap=gap, shift=shift, in_place=in_place, steps=steps, coef=coef)
+        for z in range(batch):
+            x = g[z].astype(np.float64)
+            x = x / (np.linalg.norm(x) + 1e-7)
+            for _ in range(steps):
+                gram = x @ x.T
+                x = coef[0] * x + (coef[1] * gram + coef[2] * (gram @ gram)) @ x
+            off = np.linalg.norm(got[z].astype(np.float64) - x)
+            assert off <= 1.01 * 2.0 ** -24 * np.linalg.norm(x) + 2.0 ** -150 * np.sqrt(rows * cols)
