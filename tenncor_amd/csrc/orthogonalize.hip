@@ -30,6 +30,7 @@
 
 #include <cmath>
 #include <new>
+#include <type_traits>
 
 namespace
 {
@@ -74,7 +75,7 @@ struct PrepArgs
 	uint64_t ldg, stride_g;
 	uint64_t rows, cols;
 	uint32_t parts;
-	double* sums; // [batch][parts]
+	double* sums; // [batch][parts][RANGES]
 	double eps;
 	float scale;
 	uint32_t* arrived; // [batch][arrivals], cleared here for the products that count in them
@@ -101,13 +102,18 @@ __device__ __forceinline__ double group_sum (double v, double* red)
 	return out;
 }
 
-// Sums of squares in double: an error of the norm is one of every singular value
+// Sums of squares in double: an error of the norm is one of every singular value.  The
+// square of a float is a normal double.  Those of doubles beyond 2^500 are taken of
+// v 2^-600 and those below 2^-500 of v 2^600, each into a sum of their own.
+template <typename T>
+constexpr int RANGES = std::is_same<T,double>::value ? 3 : 1; // as they are, large, small
+
 template <typename T>
 __global__ __launch_bounds__(256) void ortho_norm_k (PrepArgs<T> a)
 {
 	__shared__ double red[4];
 	const T* g = a.g + blockIdx.y * a.stride_g;
-	double sum = 0;
+	double sum[RANGES<T>] = {};
 	// runs of the rows dealt to the workgroups' waves, lanes along a run
 	const uint32_t wave = threadIdx.x / TCG_WAVE, lane = threadIdx.x & (TCG_WAVE - 1);
 	const uint64_t runs = (a.cols + NORM_RUN - 1) / NORM_RUN;
@@ -119,24 +125,65 @@ __global__ __launch_bounds__(256) void ortho_norm_k (PrepArgs<T> a)
 		for (uint64_t col = from + lane; col < to; col += TCG_WAVE)
 		{
 			const double v = p[col];
-			sum += v * v;
+			if constexpr (RANGES<T> == 1) { sum[0] += v * v; }
+			else
+			{
+				// (a NaN is neither large nor small)
+				const bool large = fabs(v) >= 0x1p500, small = fabs(v) < 0x1p-500;
+				const double w = v * (large ? 0x1p-600 : small ? 0x1p600 : 1.), square = w * w;
+				sum[0] += large || small ? 0. : square;
+				sum[1] += large ? square : 0.;
+				sum[2] += small ? square : 0.;
+			}
 		}
 	}
 	if (blockIdx.x == 0)
 	{
 		for (uint32_t i = threadIdx.x; i < a.arrivals; i += blockDim.x) { a.arrived[(uint64_t) blockIdx.y * a.arrivals + i] = 0; }
 	}
-	sum = group_sum(sum, red);
-	if (threadIdx.x == 0) { a.sums[(uint64_t) blockIdx.y * a.parts + blockIdx.x] = sum; }
+#pragma unroll
+	for (int k = 0; k < RANGES<T>; ++k)
+	{
+		const double all = group_sum(sum[k], red);
+		if (threadIdx.x == 0) { a.sums[((uint64_t) blockIdx.y * a.parts + blockIdx.x) * RANGES<T> + k] = all; }
+	}
 }
 
-/// 1 / (|G| + eps) in every lane
-template <typename T>
-__device__ __forceinline__ double inverse_norm (const PrepArgs<T>& a, uint32_t batch, double* red)
+/// X = (G shift) inverse, `shift` a power of two
+struct Normed
 {
-	double sum = 0;
-	for (uint32_t p = threadIdx.x; p < a.parts; p += blockDim.x) { sum += a.sums[(uint64_t) batch * a.parts + p]; }
-	return 1. / (::sqrt(group_sum(sum, red)) + a.eps);
+	double shift, inverse;
+
+	template <typename T>
+	__device__ __forceinline__ double operator () (T v) const { return (double) v * shift * inverse; }
+};
+
+/// The norm's part in every lane; `scale`: what X is multiplied by besides
+template <typename T>
+__device__ __forceinline__ Normed normed (const PrepArgs<T>& a, uint32_t batch, double* red, double scale)
+{
+	double sum[3] = {};
+#pragma unroll
+	for (int k = 0; k < RANGES<T>; ++k)
+	{
+		for (uint32_t p = threadIdx.x; p < a.parts; p += blockDim.x) { sum[k] += a.sums[((uint64_t) batch * a.parts + p) * RANGES<T> + k]; }
+		sum[k] = group_sum(sum[k], red);
+	}
+	double square = sum[0] + sum[2] * 0x1p-600 * 0x1p-600;
+	Normed out = {1., 0.};
+	if (sum[1] > 0)
+	{
+		square = sum[1] + sum[0] * 0x1p-600 * 0x1p-600;
+		out.shift = 0x1p-600;
+	}
+	else if (sum[0] == 0 && a.eps < 0x1p-400)
+	{
+		// nothing but small values, or zeros, whose quotient is zero for the smallest epsilon too
+		square = sum[2];
+		out.shift = 0x1p600;
+	}
+	out.inverse = 1. / (::sqrt(square) + a.eps * out.shift) * scale;
+	return out;
 }
 
 /// Where the 32 x 32 block (bi, bj) of a matrix of `rows` rows keeps its values in fp32:
@@ -176,9 +223,9 @@ __global__ __launch_bounds__(256) void ortho_split_k (PrepArgs<float> a, uint32_
 	const uint64_t r0 = (uint64_t) (blockIdx.x / tiles_x) * 64, c0 = (uint64_t) (blockIdx.x % tiles_x) * 64;
 	float v[16];
 	tile_values(v, a, a.g + batch * a.stride_g, r0, c0);
-	const double inv = inverse_norm(a, batch, red) * a.scale;
+	const Normed x = normed(a, batch, red, a.scale);
 #pragma unroll
-	for (int i = 0; i < 16; ++i) { tile[threadIdx.x / 64 + 4 * i][threadIdx.x % 64] = (float) ((double) v[i] * inv); }
+	for (int i = 0; i < 16; ++i) { tile[threadIdx.x / 64 + 4 * i][threadIdx.x % 64] = (float) x(v[i]); }
 	__syncthreads();
 	// G's rows are X's rows, or X^T's
 	f16* along = (a.tall ? a.xt + batch * a.stride_xt : a.x + batch * a.stride_x);
@@ -693,7 +740,8 @@ __global__ __launch_bounds__(1024) void ortho_small_k (SmallArgs g)
 		for (uint32_t w = 0; w < waves; ++w) { sum += red[w]; }
 		__syncthreads();
 	}
-	const double inv = (double) g.scale / (::sqrt(sum) + g.eps);
+	// (zeros stay zeros for an epsilon whose reciprocal is infinite)
+	const double inv = sum == 0 && g.eps > 0 ? 0. : (double) g.scale / (::sqrt(sum) + g.eps);
 #pragma unroll
 	for (int t = 0; t < TILES; ++t)
 	{
@@ -1011,7 +1059,7 @@ __global__ __launch_bounds__(256) void ortho_scale_k (PrepArgs<T> a, uint32_t ti
 	const uint64_t r0 = (uint64_t) (blockIdx.x / tiles_x) * 64, c0 = (uint64_t) (blockIdx.x % tiles_x) * 64;
 	T v[16];
 	tile_values(v, a, a.g + batch * a.stride_g, r0, c0);
-	const double inv = inverse_norm(a, batch, red);
+	const Normed x = normed(a, batch, red, 1.);
 	double* along = a.dense[a.tall] + batch * a.stride_dense;
 	double* across = a.dense[!a.tall] + batch * a.stride_dense;
 	const uint64_t ld_along = a.tall ? a.ldxt : a.ldx, ld_across = a.tall ? a.ldx : a.ldxt;
@@ -1019,8 +1067,8 @@ __global__ __launch_bounds__(256) void ortho_scale_k (PrepArgs<T> a, uint32_t ti
 	for (int i = 0; i < 16; ++i)
 	{
 		const uint32_t r = threadIdx.x / 64 + 4 * i, c = threadIdx.x % 64;
-		tile[r][c] = v[i] * inv;
-		along[(r0 + r) * ld_along + c0 + c] = v[i] * inv;
+		tile[r][c] = x(v[i]);
+		along[(r0 + r) * ld_along + c0 + c] = tile[r][c];
 	}
 	__syncthreads();
 #pragma unroll
@@ -1420,7 +1468,7 @@ int ortho_double (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, 
 	const uint64_t mp = padded(m, 64), np = padded(n, 64);
 	const size_t xs = (size_t) mp * np, as = (size_t) mp * mp;
 	const uint32_t parts = norm_parts(rows, cols);
-	const size_t sums_bytes = ((size_t) batch * parts * sizeof(double) + 255) / 256 * 256;
+	const size_t sums_bytes = ((size_t) batch * parts * RANGES<T> * sizeof(double) + 255) / 256 * 256;
 	const size_t bytes = sums_bytes + (4 * xs + 2 * as) * batch * sizeof(double);
 	TCG_REQUIRE(ctx, mp / 16 * (np / 16) * batch < (1ull << 31), "tcg_orthogonalize: %llu matrices of %llu x %llu are too many",
 		(unsigned long long) batch, (unsigned long long) rows, (unsigned long long) cols);
