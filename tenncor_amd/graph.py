@@ -705,8 +705,10 @@ class Approx:
     def muon(self, error, variables, learning_rate=0.02, decay=0.95, nesterov=True, steps=5, epsilon=1e-7):
         """For weight matrices: momentum = decay momentum + f'(x), and x moves along
         the orthogonalised momentum (with `nesterov` along f'(x) + decay momentum):
-        x -= learning_rate sqrt(max(1, rows / columns)) orthogonalize(...).  Not one
-        of the reference's rules; variables that are no matrices are for the others."""
+        x -= learning_rate sqrt(max(1, outputs / inputs)) orthogonalize(...), with the
+        weights of a layer as `matmul` and `dense` take them: dim 0 counts its outputs,
+        dim 1 its inputs.  Not one of the reference's rules; variables that are no
+        matrices are for the others."""
         a = self.api
         out = []
         for x in variables:
@@ -716,7 +718,7 @@ class Approx:
             momentum = self._variable_like(0, x, "momentum")
             following = a.assign(momentum, a.add(a.mul(decay, momentum), der))
             along = a.add(der, a.mul(decay, following)) if nesterov else following
-            rate = learning_rate * max(1.0, x.shape[1] / x.shape[0]) ** 0.5
+            rate = learning_rate * max(1.0, x.shape[0] / x.shape[1]) ** 0.5
             out.append((x, a.assign_sub(x, a.mul(rate, a.orthogonalize(along, steps, epsilon)))))
         return out
 
