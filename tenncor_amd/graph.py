@@ -708,11 +708,13 @@ class Approx:
         x -= learning_rate sqrt(max(1, outputs / inputs)) orthogonalize(...), with the
         weights of a layer as `matmul` and `dense` take them: dim 0 counts its outputs,
         dim 1 its inputs.  Not one of the reference's rules; variables that are no
-        matrices are for the others."""
+        matrices are for the others and refused, vectors and with them the weights of a
+        single input ({n} and {n, 1} are one shape)."""
         a = self.api
         out = []
         for x in variables:
-            if any(d != 1 for d in x.shape[2:]):
+            # a shape does not tell a vector from a matrix whose dim 1 is one
+            if x.shape[1] == 1 or any(d != 1 for d in x.shape[2:]):
                 raise ValueError("muon updates matrices, not a variable of shape %s" % x.shape)
         for x, der in zip(variables, self.g.derive(error, variables)):
             momentum = self._variable_like(0, x, "momentum")
