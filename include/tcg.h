@@ -676,7 +676,8 @@ int tcg_layer_norm (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols,
  * together costs less than one call each.  mean / rstd: what the forward
  * pass left, or both NULL, and they are taken from x again (eps is used only
  * then).  The sums over rows run in a fixed order: the same bits at every call.
- * dx may be dy or x (same leading dim).  No rows: dweight and dbias are zero. */
+ * dx may be dy or x (same leading dim), dweight or dbias may be weight.  No rows:
+ * dweight and dbias are zero. */
 int tcg_layer_norm_grad (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols,
 	const void* dy, uint64_t lddy, const void* x, uint64_t ldx, const void* weight,
 	const void* mean, const void* rstd, double eps,

@@ -930,18 +930,18 @@ int grad_chunked (tcg_ctx* ctx, const GradArgs<T>& g, uint64_t cols, double eps,
 	const unsigned row_grid = (unsigned) ((a.rows + 255) / 256);
 	if (nullptr == a.mean_in) { layer_norm_chunk_stats_k<T><<<grid, 256, 0, ctx->stream>>>(a); }
 	layer_norm_chunk_merge_k<T><<<row_grid, 256, 0, ctx->stream>>>(a);
-	// the sums over rows before dx: dx may lie where dy or x does
-	if (parts)
-	{
-		const unsigned strips = chunk_grid(ctx, (cols + 255) / 256);
-		layer_norm_chunk_params_k<T><<<dim3(strips, parts), 256, 0, ctx->stream>>>(a, partial);
-		layer_norm_chunk_params_sum_k<T><<<chunk_grid(ctx, (2 * cols + 255) / 256), 256, 0, ctx->stream>>>(partial, parts, cols, dweight, dbias);
-	}
+	// the sums over rows before dx, which may lie where dy or x does, and their results after
+	// it: these may lie where the weight does
+	if (parts) { layer_norm_chunk_params_k<T><<<dim3(chunk_grid(ctx, (cols + 255) / 256), parts), 256, 0, ctx->stream>>>(a, partial); }
 	if (a.out)
 	{
 		layer_norm_chunk_grad_sums_k<T><<<grid, 256, 0, ctx->stream>>>(a);
 		layer_norm_chunk_grad_merge_k<T><<<row_grid, 256, 0, ctx->stream>>>(a);
 		layer_norm_chunk_dx_k<T><<<grid, 256, 0, ctx->stream>>>(a);
+	}
+	if (parts)
+	{
+		layer_norm_chunk_params_sum_k<T><<<chunk_grid(ctx, (2 * cols + 255) / 256), 256, 0, ctx->stream>>>(partial, parts, cols, dweight, dbias);
 	}
 	hipError_t err = hipGetLastError();
 	rc = tcg_free(ctx, mem, bytes);
@@ -1000,8 +1000,15 @@ int grad_run (tcg_ctx* ctx, uint64_t rows, uint64_t cols, const void* dy, uint64
 	a.cols = (uint32_t) cols;
 	a.eps = (T) eps;
 	a.inv_n = (T) (1. / (double) cols);
-	// one launch for a few rows; dx must not lie where dw's sums still read
-	if (dx && (dweight || dbias) && mean && dx != x && dx != dy && cols >= VN<T> && shape.span <= 256 && rows <= FEW_ROWS)
+	// one launch for a few rows; dx must not lie where dw's sums still read, nor dw or db where
+	// dx still reads the weight
+	const auto beside_weight = [&] (const void* p)
+	{
+		const uintptr_t at = (uintptr_t) p, w = (uintptr_t) weight, bytes = cols * sizeof(T);
+		return !p || !weight || (at > w ? at - w : w - at) >= bytes;
+	};
+	if (dx && (dweight || dbias) && mean && dx != x && dx != dy && beside_weight(dweight) && beside_weight(dbias) &&
+		cols >= VN<T> && shape.span <= 256 && rows <= FEW_ROWS)
 	{
 		switch (shape.span)
 		{
