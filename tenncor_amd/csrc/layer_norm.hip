@@ -150,19 +150,20 @@ __device__ __forceinline__ float fused (float a, float b, float c) { return __bu
 __device__ __forceinline__ double fused (double a, double b, double c) { return __builtin_fma(a, b, c); }
 
 /// v / n by way of inv_n = 1 / n rounded: the remainder puts the last bit right, so that
-/// a quotient that is a number of the type comes out as that (41 x (1 / 41) does not)
+/// a quotient that is a number of the type comes out as that (41 x (1 / 41) does not).
+/// Not for infinite v.
 template <typename T>
 __device__ __forceinline__ T quotient (T v, T n, T inv_n)
 {
 	const T q = rounded(v, inv_n);
-	return fabs(q) <= std::numeric_limits<T>::max() ? fused(fused(-q, n, v), inv_n, q) : q;
+	return fused(fused(-q, n, v), inv_n, q);
 }
 
 /// Mean and reciprocal deviation of the row held in v (PER vectors a lane); what
 /// is left of a value after the mean is (x - m) - c, see above.  In a row of equal elements
-/// all sums but the first are exact, and so are both quotients: nothing is left, and the
-/// variance is zero.  (With products by inv_n 83 elements of 16.2 came to -4e-11 in place of 0
-/// and 141 of 1.9e7 to -4e-5.)
+/// all sums but the first are exact, and so are c and c ds: nothing is left, and the variance
+/// is zero.  (With c = ds inv_n 83 elements of 16.2 came to -4e-11 in place of 0 and 141 of
+/// 1.9e7 to -4e-5.)  Where the sum of squares is infinite r is zero.
 template <typename T, int SPAN, int PER, bool RAGGED>
 __device__ __forceinline__ void row_stats (const typename Vec16<T>::type (&v)[PER], uint32_t lane, uint32_t cols, T inv_n, T eps,
 	T* red, uint32_t& turn, T& m, T& c, T& r)
@@ -190,9 +191,8 @@ __device__ __forceinline__ void row_stats (const typename Vec16<T>::type (&v)[PE
 		}
 	}
 	row_sums<T,SPAN>(ds, dq, red, turn);
-	const T n = (T) cols;
-	c = quotient(ds, n, inv_n);
-	T var = quotient(dq, n, inv_n) - c * c;
+	c = quotient(ds, (T) cols, inv_n);
+	T var = fused(-c, ds, dq) * inv_n;
 	var = var < 0 ? (T) 0 : var;
 	r = inv_sqrt(var + eps);
 }
