@@ -90,16 +90,29 @@ struct PrepArgs
 	bool tall; // X = G^T
 };
 
-__device__ __forceinline__ double group_sum (double v, double* red)
+/// N values summed over the workgroup at once, in every lane
+template <int N>
+__device__ __forceinline__ void group_sums (double (&v)[N], double* red)
 {
 #pragma unroll
-	for (int d = TCG_WAVE / 2; d > 0; d >>= 1) { v += __shfl_xor(v, d); }
-	if ((threadIdx.x & (TCG_WAVE - 1)) == 0) { red[threadIdx.x / TCG_WAVE] = v; }
+	for (int d = TCG_WAVE / 2; d > 0; d >>= 1)
+	{
+#pragma unroll
+		for (int k = 0; k < N; ++k) { v[k] += __shfl_xor(v[k], d); }
+	}
+	if ((threadIdx.x & (TCG_WAVE - 1)) == 0)
+	{
+#pragma unroll
+		for (int k = 0; k < N; ++k) { red[threadIdx.x / TCG_WAVE * N + k] = v[k]; }
+	}
 	__syncthreads();
-	double out = 0;
-	for (uint32_t w = 0; w < blockDim.x / TCG_WAVE; ++w) { out += red[w]; }
+#pragma unroll
+	for (int k = 0; k < N; ++k)
+	{
+		v[k] = 0;
+		for (uint32_t w = 0; w < blockDim.x / TCG_WAVE; ++w) { v[k] += red[w * N + k]; }
+	}
 	__syncthreads();
-	return out;
 }
 
 // Sums of squares in double: an error of the norm is one of every singular value.  The
@@ -111,7 +124,7 @@ constexpr int RANGES = std::is_same<T,double>::value ? 3 : 1; // as they are, la
 template <typename T>
 __global__ __launch_bounds__(256) void ortho_norm_k (PrepArgs<T> a)
 {
-	__shared__ double red[4];
+	__shared__ double red[4 * RANGES<T>];
 	const T* g = a.g + blockIdx.y * a.stride_g;
 	double sum[RANGES<T>] = {};
 	// runs of the rows dealt to the workgroups' waves, lanes along a run
@@ -141,11 +154,11 @@ __global__ __launch_bounds__(256) void ortho_norm_k (PrepArgs<T> a)
 	{
 		for (uint32_t i = threadIdx.x; i < a.arrivals; i += blockDim.x) { a.arrived[(uint64_t) blockIdx.y * a.arrivals + i] = 0; }
 	}
-#pragma unroll
-	for (int k = 0; k < RANGES<T>; ++k)
+	group_sums(sum, red);
+	if (threadIdx.x == 0)
 	{
-		const double all = group_sum(sum[k], red);
-		if (threadIdx.x == 0) { a.sums[((uint64_t) blockIdx.y * a.parts + blockIdx.x) * RANGES<T> + k] = all; }
+#pragma unroll
+		for (int k = 0; k < RANGES<T>; ++k) { a.sums[((uint64_t) blockIdx.y * a.parts + blockIdx.x) * RANGES<T> + k] = sum[k]; }
 	}
 }
 
@@ -162,25 +175,29 @@ struct Normed
 template <typename T>
 __device__ __forceinline__ Normed normed (const PrepArgs<T>& a, uint32_t batch, double* red, double scale)
 {
-	double sum[3] = {};
+	double sum[RANGES<T>] = {};
+	for (uint32_t p = threadIdx.x; p < a.parts; p += blockDim.x)
+	{
 #pragma unroll
-	for (int k = 0; k < RANGES<T>; ++k)
-	{
-		for (uint32_t p = threadIdx.x; p < a.parts; p += blockDim.x) { sum[k] += a.sums[((uint64_t) batch * a.parts + p) * RANGES<T> + k]; }
-		sum[k] = group_sum(sum[k], red);
+		for (int k = 0; k < RANGES<T>; ++k) { sum[k] += a.sums[((uint64_t) batch * a.parts + p) * RANGES<T> + k]; }
 	}
-	double square = sum[0] + sum[2] * 0x1p-600 * 0x1p-600;
+	group_sums(sum, red);
+	double square = sum[0];
 	Normed out = {1., 0.};
-	if (sum[1] > 0)
+	if constexpr (RANGES<T> > 1)
 	{
-		square = sum[1] + sum[0] * 0x1p-600 * 0x1p-600;
-		out.shift = 0x1p-600;
-	}
-	else if (sum[0] == 0 && a.eps < 0x1p-400)
-	{
-		// nothing but small values, or zeros, whose quotient is zero for the smallest epsilon too
-		square = sum[2];
-		out.shift = 0x1p600;
+		square += sum[2] * 0x1p-600 * 0x1p-600;
+		if (sum[1] > 0)
+		{
+			square = sum[1] + sum[0] * 0x1p-600 * 0x1p-600;
+			out.shift = 0x1p-600;
+		}
+		else if (sum[0] == 0 && a.eps < 0x1p-400)
+		{
+			// nothing but small values, or zeros, whose quotient is zero for the smallest epsilon too
+			square = sum[2];
+			out.shift = 0x1p600;
+		}
 	}
 	out.inverse = 1. / (::sqrt(square) + a.eps * out.shift) * scale;
 	return out;
@@ -217,7 +234,7 @@ __device__ __forceinline__ void tile_values (T (&v)[16], const PrepArgs<T>& a, c
 // lies outside G is zero
 __global__ __launch_bounds__(256) void ortho_split_k (PrepArgs<float> a, uint32_t tiles_x)
 {
-	__shared__ double red[4];
+	__shared__ double red[4 * RANGES<float>];
 	__shared__ float tile[64][65];
 	const uint32_t batch = blockIdx.y;
 	const uint64_t r0 = (uint64_t) (blockIdx.x / tiles_x) * 64, c0 = (uint64_t) (blockIdx.x % tiles_x) * 64;
@@ -740,8 +757,7 @@ __global__ __launch_bounds__(1024) void ortho_small_k (SmallArgs g)
 		for (uint32_t w = 0; w < waves; ++w) { sum += red[w]; }
 		__syncthreads();
 	}
-	// (zeros stay zeros for an epsilon whose reciprocal is infinite)
-	const double inv = sum == 0 && g.eps > 0 ? 0. : (double) g.scale / (::sqrt(sum) + g.eps);
+	const double inv = (double) g.scale / (::sqrt(sum) + g.eps);
 #pragma unroll
 	for (int t = 0; t < TILES; ++t)
 	{
@@ -1053,7 +1069,7 @@ __global__ __launch_bounds__(256) void ortho_double_k (DoubleArgs g)
 template <typename T>
 __global__ __launch_bounds__(256) void ortho_scale_k (PrepArgs<T> a, uint32_t tiles_x)
 {
-	__shared__ double red[4];
+	__shared__ double red[4 * RANGES<T>];
 	__shared__ double tile[64][65];
 	const uint32_t batch = blockIdx.y;
 	const uint64_t r0 = (uint64_t) (blockIdx.x / tiles_x) * 64, c0 = (uint64_t) (blockIdx.x % tiles_x) * 64;
@@ -1593,6 +1609,9 @@ int tcg_orthogonalize (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols, ui
 		TCG_REQUIRE(ctx, follow(plan), "tcg_orthogonalize: with the polynomial %g s + %g s^3 + %g s^5 singular values grow past 1e6",
 			coef[0], coef[1], coef[2]);
 		if (batch == 1) { stride_i = stride_o = 0; }
+		// beside the norm of a matrix of floats, 1e-45 or more, this is nothing either, and its
+		// reciprocal, by which zeros are multiplied, is finite
+		if (dtype == TCG_FLOAT && eps > 0 && eps < 0x1p-900) { eps = 0x1p-900; }
 		if (dtype == TCG_DOUBLE) { return ortho_double(ctx, plan, rows, cols, batch, (const double*) in, ldi, stride_i, eps, (double*) out, ldo, stride_o); }
 		return halves_hold(plan) ?
 			ortho_float(ctx, plan, rows, cols, batch, (const float*) in, ldi, stride_i, eps, (float*) out, ldo, stride_o) :
