@@ -684,7 +684,8 @@ int tcg_layer_norm_grad (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols,
 	void* dx, uint64_t lddx, void* dweight, void* dbias);
 
 /* The orthogonalised update of weight matrices: `batch` matrices of rows x cols
- * elements (matrix z, row i at in + z * stride_i + i * ldi), each by itself
+ * elements (matrix z, row i at in + z * stride_i + i * ldi: one behind the other, or
+ * side by side as column blocks of a wider matrix), each by itself
  *   X = G / (|G| + eps), |G| the root of the sum of its squares,
  *   A = X X^T    B = coef[1] A + coef[2] A A    X <- coef[0] X + B X
  * `steps` times (with the transposed of X where rows > cols, which gives the

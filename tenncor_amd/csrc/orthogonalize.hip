@@ -1570,6 +1570,7 @@ int ortho_double (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, 
 
 constexpr uint64_t MOST_ELEMENTS = 1ull << 33; // of one matrix, padding included; its temporaries take up to 32 bytes an element
 constexpr uint64_t MOST_BATCH = 65535;
+constexpr uint64_t MOST_APART = 1ull << 40; // elements from the first matrix to the last: more than any memory holds
 
 } // namespace
 
@@ -1591,8 +1592,15 @@ int tcg_orthogonalize (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols, ui
 		padded(rows, 128) <= MOST_ELEMENTS / padded(cols, 128) && batch <= MOST_BATCH,
 		"tcg_orthogonalize: %llu matrices of %llu x %llu are too many or too large",
 		(unsigned long long) batch, (unsigned long long) rows, (unsigned long long) cols);
-	// a matrix's rows end before the next matrix begins
-	const auto apart = [&] (uint64_t ld, uint64_t stride) { return batch == 1 || stride >= (rows - 1) * ld + cols; };
+	TCG_REQUIRE(ctx, batch == 1 || (stride_i <= MOST_APART / (batch - 1) && stride_o <= MOST_APART / (batch - 1)),
+		"tcg_orthogonalize: %llu matrices %llu and %llu elements from one to the next are too far apart",
+		(unsigned long long) batch, (unsigned long long) stride_i, (unsigned long long) stride_o);
+	// a matrix's rows end before the next matrix begins, or the matrices lie side by side in
+	// rows that hold one of each
+	const auto apart = [&] (uint64_t ld, uint64_t stride)
+	{
+		return batch == 1 || stride >= (rows - 1) * ld + cols || (stride >= cols && stride <= ld && (batch - 1) * stride <= ld - cols);
+	};
 	TCG_REQUIRE(ctx, apart(ldi, stride_i) && apart(ldo, stride_o), "tcg_orthogonalize: matrices %llu and %llu elements apart overlap",
 		(unsigned long long) stride_i, (unsigned long long) stride_o);
 	TCG_REQUIRE(ctx, in != out || (ldi == ldo && (batch == 1 || stride_i == stride_o)),
