@@ -811,8 +811,9 @@ void norm_launch_per (tcg_ctx* ctx, const NormArgs<T>& a, int per)
 	{
 		case 1: norm_launch<T,SPAN,1>(ctx, a); break;
 		case 2: norm_launch<T,SPAN,2>(ctx, a); break;
-		case 4: norm_launch<T,SPAN,4>(ctx, a); break;
-		default: norm_launch<T,SPAN,8>(ctx, a); break;
+		case 8: // the longest rows only, see norm_run
+			if constexpr (SPAN == 1024) { norm_launch<T,SPAN,8>(ctx, a); break; }
+		default: norm_launch<T,SPAN,4>(ctx, a); break;
 	}
 }
 
