@@ -662,9 +662,11 @@ int tcg_conv_route_counts (const tcg_ctx* ctx, uint64_t* patch, uint64_t* short_
  * tcg_layer_norm_grad takes).  float and double; a row's sums are taken in the
  * type of x, the mean with a correction for its own rounding.  A row of equal
  * elements gives bias (with eps = 0: NaN, as the formula says); infinities and
- * NaN stay in their row.  y may be x (same leading dim).  No rows: nothing is
- * done.  The reference has no such operator: cfg/tenncor/core.yml composes it
- * from reduce_mean, sub, square, sqrt and div. */
+ * NaN stay in their row.  A row whose sum leaves the range of the type gives NaN, one
+ * whose deviations' squares do (deviations of 1e19 in float) bias and a zero in rstd.
+ * y may be x (same leading dim).  No rows: nothing is done.  The reference has no
+ * such operator: cfg/tenncor/core.yml composes it from reduce_mean, sub, square,
+ * sqrt and div. */
 int tcg_layer_norm (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols,
 	const void* x, uint64_t ldx, const void* weight, const void* bias, double eps,
 	void* y, uint64_t ldy, void* mean, void* rstd);
@@ -675,7 +677,8 @@ int tcg_layer_norm (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols,
  * Each of dx, dweight and dbias may be NULL (not all three); what is wanted
  * together costs less than one call each.  mean / rstd: what the forward
  * pass left, or both NULL, and they are taken from x again (eps is used only
- * then).  The sums over rows run in a fixed order: the same bits at every call.
+ * then; a mean given is one rounded to the type, which shows in rows far from
+ * zero).  The sums over rows run in a fixed order: the same bits at every call.
  * dx may be dy or x (same leading dim), dweight or dbias may be weight.  No rows:
  * dweight and dbias are zero. */
 int tcg_layer_norm_grad (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols,

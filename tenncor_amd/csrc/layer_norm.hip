@@ -1080,6 +1080,13 @@ bool sizes_fit (uint64_t rows, uint64_t ld)
 	return ld == 0 || rows <= MOST_ELEMENTS / ld;
 }
 
+/// An epsilon above zero stays above zero in the type of the rows
+double kept_eps (int dtype, double eps)
+{
+	const double least = std::numeric_limits<float>::denorm_min();
+	return dtype == TCG_FLOAT && eps > 0 && eps < least ? least : eps;
+}
+
 } // namespace
 
 extern "C" {
@@ -1100,6 +1107,7 @@ int tcg_layer_norm (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols, const
 		(unsigned long long) ldx, (unsigned long long) ldy);
 	if (tcg_small_mode(ctx)) { TCG_SMALL_RETURN(ctx, tcg_small_unsupported(ctx, "a layer normalisation")); }
 	if (0 == rows) { return TCG_OK; }
+	eps = kept_eps(dtype, eps);
 	tcg_device_scope device(ctx);
 	return dtype == TCG_FLOAT ? norm_run<float>(ctx, rows, cols, x, ldx, weight, bias, eps, y, ldy, mean, rstd) :
 		norm_run<double>(ctx, rows, cols, x, ldx, weight, bias, eps, y, ldy, mean, rstd);
@@ -1124,6 +1132,7 @@ int tcg_layer_norm_grad (tcg_ctx* ctx, int dtype, uint64_t rows, uint64_t cols, 
 	TCG_REQUIRE(ctx, !dx || ((dx != dy || lddx == lddy) && (dx != x || lddx == ldx)),
 		"tcg_layer_norm_grad: dx in place of an operand with another leading dim");
 	if (tcg_small_mode(ctx)) { TCG_SMALL_RETURN(ctx, tcg_small_unsupported(ctx, "the gradients of a layer normalisation")); }
+	eps = kept_eps(dtype, eps);
 	tcg_device_scope device(ctx);
 	if (0 == rows)
 	{

@@ -53,3 +53,17 @@ def test_deviations_that_cannot_be_squared(ctx, cols):
     if cols < 33000:
         np.testing.assert_array_equal(y, np.repeat(b[None], 3, 0))
         assert not rstd.any()
+
+
+@pytest.mark.parametrize("t", [np.float32, np.float64])
+@pytest.mark.parametrize("cols", [5, 83, 5000, 40001])
+def test_the_smallest_epsilon_is_one(ctx, cols, t):
+    """Below the type's numbers too: h is 0, and with it dweight."""
+    rng = np.random.default_rng(cols)
+    x = np.repeat(rng.uniform(1, 2, 4).astype(t)[:, None], cols, 1)
+    b, g = rng.normal(0, 1, cols).astype(t), rng.normal(0, 1, x.shape).astype(t)
+    for eps in (1e-50, 1e-310, 5e-324):
+        y, _, rstd = run_forward(ctx, x, None, b, eps)
+        np.testing.assert_array_equal(y, np.repeat(b[None], 4, 0))
+        assert np.isfinite(rstd).all()
+        assert not run_backward(ctx, g, x, None, eps, want=("dw",))["dw"].any()
