@@ -165,7 +165,7 @@ __device__ __forceinline__ T quotient (T v, T n, T inv_n)
 /// is zero.  (With c = ds inv_n 83 elements of 16.2 came to -4e-11 in place of 0 and 141 of
 /// 1.9e7 to -4e-5.)  Where the sum of squares is infinite r is zero.
 template <typename T, int SPAN, int PER, bool RAGGED>
-__device__ __forceinline__ void row_stats (const typename Vec16<T>::type (&v)[PER], uint32_t lane, uint32_t cols, T inv_n, T eps,
+__device__ __forceinline__ void row_stats (const typename Vec16<T>::type (&v)[PER], uint32_t lane, uint32_t cols, T n, T inv_n, T eps,
 	T* red, uint32_t& turn, T& m, T& c, T& r)
 {
 	T sum = 0, none = 0;
@@ -191,7 +191,7 @@ __device__ __forceinline__ void row_stats (const typename Vec16<T>::type (&v)[PE
 		}
 	}
 	row_sums<T,SPAN>(ds, dq, red, turn);
-	c = quotient(ds, (T) cols, inv_n);
+	c = quotient(ds, n, inv_n);
 	T var = fused(-c, ds, dq) * inv_n;
 	var = var < 0 ? (T) 0 : var;
 	r = inv_sqrt(var + eps);
@@ -217,7 +217,7 @@ struct NormArgs
 	T* rstd;
 	uint64_t rows;
 	uint32_t cols;
-	T eps, inv_n;
+	T eps, n, inv_n; // n: cols, in a scalar register next to its reciprocal
 };
 
 /// Workgroups of 256 lanes take several rows at once; a row of more lanes has one to itself
@@ -251,7 +251,7 @@ __global__ __launch_bounds__(group_size(SPAN)) void layer_norm_k (NormArgs<T> a)
 #pragma unroll
 		for (int j = 0; j < PER; ++j) { v[j] = load_vec<T,RAGGED>(x, (j * SPAN + lane) * VN<T>, a.cols); }
 		T m, c, r;
-		row_stats<T,SPAN,PER,RAGGED>(v, lane, a.cols, a.inv_n, a.eps, red, turn, m, c, r);
+		row_stats<T,SPAN,PER,RAGGED>(v, lane, a.cols, a.n, a.inv_n, a.eps, red, turn, m, c, r);
 		T* y = a.y + row * a.ldy;
 #pragma unroll
 		for (int j = 0; j < PER; ++j)
@@ -284,7 +284,7 @@ struct GradArgs
 	T* partial;      // [workgroup][dw, db][cols]
 	uint64_t rows;
 	uint32_t cols;
-	T eps, inv_n;
+	T eps, n, inv_n; // n: cols, in a scalar register next to its reciprocal
 };
 
 // ONCE: x, dy and dx are more than the caches hold.
@@ -325,7 +325,7 @@ __device__ __forceinline__ void grad_rows (const GradArgs<T>& a, uint32_t group,
 			m = a.mean[row];
 			r = a.rstd[row];
 		}
-		else { row_stats<T,SPAN,PER,RAGGED>(h, lane, a.cols, a.inv_n, a.eps, red, turn, m, c, r); }
+		else { row_stats<T,SPAN,PER,RAGGED>(h, lane, a.cols, a.n, a.inv_n, a.eps, red, turn, m, c, r); }
 		T sg = 0, sh = 0;
 #pragma unroll
 		for (int j = 0; j < PER; ++j)
@@ -560,7 +560,7 @@ __global__ __launch_bounds__(256) void layer_norm_chunk_stats_k (ChunkArgs<T> a)
 #pragma unroll
 		for (uint32_t j = 0; j < CHUNK_VECS; ++j) { v[j] = load_vec<T,true>(x, (j * 256 + threadIdx.x) * VN<T>, count); }
 		T m, c, r;
-		row_stats<T,256,CHUNK_VECS,true>(v, threadIdx.x, count, (T) 1 / (T) count, (T) 0, red, turn, m, c, r);
+		row_stats<T,256,CHUNK_VECS,true>(v, threadIdx.x, count, (T) count, (T) 1 / (T) count, (T) 0, red, turn, m, c, r);
 		T dq = 0, none = 0;
 #pragma unroll
 		for (uint32_t j = 0; j < CHUNK_VECS; ++j)
@@ -983,6 +983,7 @@ int norm_run (tcg_ctx* ctx, uint64_t rows, uint64_t cols, const void* x, uint64_
 	if (0 == shape.span) { return norm_chunked(ctx, a, cols, eps); }
 	a.cols = (uint32_t) cols;
 	a.eps = (T) eps;
+	a.n = (T) cols;
 	a.inv_n = (T) (1. / (double) cols);
 	switch (shape.span)
 	{
@@ -1016,6 +1017,7 @@ int grad_run (tcg_ctx* ctx, uint64_t rows, uint64_t cols, const void* dy, uint64
 	if (0 == shape.span) { return grad_chunked(ctx, a, cols, eps, (T*) dweight, (T*) dbias); }
 	a.cols = (uint32_t) cols;
 	a.eps = (T) eps;
+	a.n = (T) cols;
 	a.inv_n = (T) (1. / (double) cols);
 	// one launch for a few rows; dx must not lie where dw's sums still read, nor dw or db where
 	// dx still reads the weight
