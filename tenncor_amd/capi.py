@@ -560,8 +560,9 @@ class Context:
 
     def orthogonalize(self, dtype, rows, cols, batch, src, ldi, stride_i, dst, ldo, stride_o, steps=5,
                       coef=(3.4445, -4.7750, 2.0315), eps=1e-7):
-        """The default coefficients take every singular value above 1e-2 of the norm to
-        between 0.68 and 1.13 in five steps."""
+        """Matrices one behind the other, or side by side in rows that hold one of each
+        (stride_i = cols, ldi = batch cols).  The default coefficients take every
+        singular value above 1e-2 of the norm to between 0.68 and 1.14 in five steps."""
         if len(coef) != 3:
             raise ValueError("coefficients of s, s^3 and s^5, not %d of them" % len(coef))
         self._check(self.lib.tcg_orthogonalize(self.handle, dtype, rows, cols, batch, src, ldi, stride_i, steps,

@@ -997,9 +997,13 @@ int norm_run (tcg_ctx* ctx, uint64_t rows, uint64_t cols, const void* x, uint64_
 	return TCG_OK;
 }
 
-// All gradients in one launch, and in two: 256 x 512 4.6 and 6.7-7.3 us, 512 x 4096 9.6 and
-// 16.7, 768 x 3000 11.4 and 13.3; 1024 x 2048 14.2 and 11.9, 2048 x 512 10.2 and 8.1.  (Rows of
-// 1024 lanes: 200 x 8192 8.7 and 13.1, but 768 x 8192 26 and 20, 500 x 16000 36 and 30.)
+// All gradients in one launch, and in two, calls one behind the other (us): 256 x 64 5.7 and
+// 8.0, 768 x 512 5.8 and 8.1, 768 x 777 5.2 and 8.8, 500 x 4096 9.7 and 16.2, 768 x 4096 13.0 and
+// 14.5, but 768 x 2048 10.9 and 10.1.  Beyond: 1024 x 64 6.3 and 8.0, 1024 x 512 6.7 and 8.2,
+// 1500 x 512 8.7 and 8.6, 1500 x 777 10.1 and 10.5, but 1024 x 2048 14.2 and 11.6, 1024 x 4096
+// 16.9 and 15.9, 2048 x 64 9.5 and 8.0: the two cross near 700 rows of 2048 elements and 1500
+// of 512, and one number of rows stands for all of them.  Rows of 1024 lanes are left to two
+// launches: 200 x 8192 would be 8.7 and 13.1, but 768 x 8192 26 and 20, 500 x 16000 36 and 30.
 constexpr uint64_t FEW_ROWS = 768;
 
 template <typename T>
@@ -1041,8 +1045,10 @@ int grad_run (tcg_ctx* ctx, uint64_t rows, uint64_t cols, const void* dy, uint64
 	}
 	const uint64_t at_once = rows_at_once(shape.span), groups = (rows + at_once - 1) / at_once;
 	const bool params = dweight || dbias;
-	// with the sums over rows every workgroup leaves a partial row behind: no more
-	// of them than fill the chip
+	// with the sums over rows every workgroup leaves a partial row behind: no more of them
+	// than fill the chip.  One, two, three and four a CU (us): 3000 x 512 8.9 9.3 10.1 10.1, 8000 x
+	// 512 14.8 14.1 13.9 15.2, 3000 x 777 13.0 12.8 14.2 14.3, 8000 x 777 24.4 22.5 21.1 25.9, 3000
+	// x 2048 20.7 19.0 19.5 20.0, 16384 x 1024 37.7 35.6 36.4 37.1, 32768 x 4096 313 264 295 288
 	const uint64_t most = (uint64_t) ctx->num_cus * (params ? (shape.span == 1024 ? 1 : 2) : 32);
 	// as many workgroups as make equal shares of the rows
 	const uint64_t share = (groups + most - 1) / most;

@@ -13,10 +13,11 @@
 // hi = half(x s), lo = half(x s - hi) and a power of two s that puts the largest
 // value the matrix can hold (the host follows the polynomial from |x| <= 1) at
 // 2^15.  Each conversion is off by 2^-11 of what it converts at most, so 2^-22 of
-// the value is lost in the worst case.  A product is hi hi + hi lo + lo hi with the
-// sums in fp32; lo lo would be 2^-22 of the product.  Three half-precision matrix
-// instructions (2.5 PFLOP/s / 3) stand for one fp32 instruction (0.157 PFLOP/s),
-// and one load of hi and lo feeds three of them.
+// the value is lost in the worst case, or, where lo is too small for that, half a
+// step of the smallest halves, 2^-25: 2^-39 of the largest value.  A product is
+// hi hi + hi lo + lo hi with the sums in fp32; lo lo would be 2^-22 of the product.
+// Three half-precision matrix instructions (2.5 PFLOP/s / 3) stand for one fp32
+// instruction (0.157 PFLOP/s), and one load of hi and lo feeds three of them.
 //
 // What an error of X does is multiplied by up to a in each later step along the
 // weak directions of G, while one of A is read through B, which is small against
@@ -1568,7 +1569,7 @@ int ortho_double (tcg_ctx* ctx, const Plan& plan, uint64_t rows, uint64_t cols, 
 	return rc;
 }
 
-constexpr uint64_t MOST_ELEMENTS = 1ull << 33; // of one matrix, padding included; its temporaries take up to 32 bytes an element
+constexpr uint64_t MOST_ELEMENTS = 1ull << 33; // of one matrix, padding included; its temporaries take up to 48 bytes an element
 constexpr uint64_t MOST_BATCH = 65535;
 constexpr uint64_t MOST_APART = 1ull << 40; // elements from the first matrix to the last: more than any memory holds
 
