@@ -76,10 +76,12 @@ static teq::RankT norm_rank (_GENERATED_OPCODE opcode, const marsh::Maps& attrs)
 {
 	teq::RankT rank;
 	eigen::Packer<teq::RankT>().unpack(rank, attrs);
-	if (0 == rank || rank >= teq::rank_cap)
+	// the number itself: as a rank 257 would be 1
+	const int64_t dims = dynamic_cast<const marsh::iNumber*>(attrs.get_attr(eigen::Packer<teq::RankT>().get_key()))->to_int64();
+	if (dims < 1 || dims >= teq::rank_cap)
 	{
-		global::throw_errf("cannot %s over %d dims: 1 to %d are possible", name_op(opcode).c_str(),
-			(int) rank, (int) teq::rank_cap - 1);
+		global::throw_errf("cannot %s over %lld dims: 1 to %d are possible", name_op(opcode).c_str(),
+			(long long) dims, (int) teq::rank_cap - 1);
 	}
 	eigen::RealsT reals;
 	eigen::Packer<eigen::RealsT>().unpack(reals, attrs);
