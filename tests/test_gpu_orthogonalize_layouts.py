@@ -3,7 +3,7 @@ recurrent cell lie in its fused weight."""
 import numpy as np
 import pytest
 
-from test_gpu_orthogonalize import CODE, MARK, ctx, gradient, run  # noqa: F401 (ctx is a fixture)
+from test_gpu_orthogonalize import CODE, MARK, ctx, gradient, reference, run  # noqa: F401 (ctx is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +66,17 @@ def test_matrices_that_do_overlap_are_refused(ctx):
             call(**args)
     ctx.sync()
     assert not a.get().any() and not b.get().any()
+
+
+@pytest.mark.parametrize("tall", [False, True])
+def test_offsets_past_32_bits(ctx, tall):
+    """Two rows of 17 million: 2.2e9 halves of a padded X, 8.7e9 bytes.  Every sum of A runs over
+    six additions in each of 2076 slabs (531250 shared by 256 workgroups): 0.25 sqrt(12456) =
+    28 * 2^-24 in the mean, twice that is allowed; the other roundings, at most 12 * 2^-24 a step
+    as derived in test_gpu_orthogonalize_kernels, count besides."""
+    rng = np.random.default_rng(1)
+    g = (rng.normal(0, 1, (2, 2)) @ rng.normal(0, 1, (2, 17_000_000))).astype(np.float32)
+    want, size = reference(g, 2)
+    got = run(ctx, (g.T.copy() if tall else g)[None], steps=2)[0]
+    off = np.linalg.norm((got.T if tall else got) - want)
+    assert off <= (56 + 12) * 2.0 ** -24 * size
